@@ -163,6 +163,11 @@ int encode_f32_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols
   return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, rows, cols, ld, box_rows, box_cols);
 }
 
+int encode_8bit_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows,
+                   int box_cols) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, cols, ld, box_rows, box_cols);
+}
+
 }  // namespace frx
 
 extern "C" int frx_abi_version(void) { return FRX_ABI_VERSION; }

@@ -276,6 +276,9 @@ namespace frx {
 //            4 stages, one 512-column accumulator; A is re-read half as often, which matters for
 //            the backward GEMMs whose K (= vocabulary or batch) is long enough to hide the
 //            epilogue.
+// kI8 (with kNH = 1, K-major operands): signed 8-bit operands, kind::i8, int32 accumulators. A
+// 128-byte sub-tile row then holds 128 K elements instead of 64 and one MMA covers K = 32 instead
+// of 16: the same bytes per stage, twice the products.
 // Either way a stage is 8 MMAs per tcgen05.commit: every commit costs the tensor pipe a drain
 // bubble of roughly one MMA, which at 4 MMAs per commit held the pipe to ~79% busy and at 8 lets
 // it run at ~99%.
@@ -299,12 +302,14 @@ struct PairCfg {
   static constexpr int kTileN = 256 * kNH;
 };
 
-template <bool kAMN, bool kBMN, int kNH, class Epi>
+template <bool kAMN, bool kBMN, int kNH, class Epi, bool kI8 = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                              TileSched sched, int num_k_blocks, const __grid_constant__ typename Epi::Params ep,
                              int* status) {
   using Cfg = PairCfg<kNH>;
+  static_assert(!kI8 || (!kAMN && !kBMN && kNH == 1), "8-bit operands are K-major in 256 x 256 tiles");
+  constexpr int kSubK = kI8 ? 128 : 64;  // K elements of one 128-byte sub-tile row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_a = smem;
@@ -388,7 +393,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
           uint8_t* db = s_b + stage * Cfg::kBBytes;
 #pragma unroll
           for (int ks = 0; ks < Cfg::kKS; ++ks) {
-            const int kk = kb * Cfg::kStageK + 64 * ks;
+            const int kk = (kb * Cfg::kKS + ks) * kSubK;
             uint8_t* da_s = da + ks * kPairSubBytes;
             if (kAMN) {
 #pragma unroll
@@ -431,10 +436,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (even CTA)
     if (lane == 0 && leader) {
-      const uint32_t idesc = make_idesc_f32acc(2 * kBM, 256, kAMN, kBMN, sched.f16 != 0);
+      const uint32_t idesc =
+          kI8 ? make_idesc_i8(2 * kBM, 256) : make_idesc_f32acc(2 * kBM, 256, kAMN, kBMN, sched.f16 != 0);
       constexpr uint32_t a_lbo = kAMN ? kMNBoxBytes : 16;
       constexpr uint32_t b_lbo = kBMN ? kMNBoxBytes : 16;
-      constexpr uint32_t a_kstep = kAMN ? 16 * 128 : 32;  // bytes per UMMA_K (= 16) step
+      constexpr uint32_t a_kstep = kAMN ? 16 * 128 : 32;  // bytes per UMMA_K (= 16, or 32 of 8 bits) step
       constexpr uint32_t b_kstep = kBMN ? 16 * 128 : 32;
       int stage = 0;
       uint32_t phase = 0;
@@ -470,7 +476,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
               for (int h = 0; h < kNH; ++h) {
                 const uint64_t bdesc =
                     make_smem_desc_sw128(b_addr + (ks * kNH + h) * kPairSubBytes + k * b_kstep, b_lbo, 1024);
-                umma_f16_pair(d_tmem + static_cast<uint32_t>(h * 256), adesc, bdesc, idesc, acc);
+                if (kI8)
+                  umma_i8_pair(d_tmem + static_cast<uint32_t>(h * 256), adesc, bdesc, idesc, acc);
+                else
+                  umma_f16_pair(d_tmem + static_cast<uint32_t>(h * 256), adesc, bdesc, idesc, acc);
               }
             }
           }

@@ -78,6 +78,10 @@ int encode_16bit_2d(CUtensorMap* map, bool f16, const void* base, int64_t rows, 
 int encode_f32_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows,
                   int box_cols);
 
+// Same for a matrix of 8-bit values (box_cols == 128).
+int encode_8bit_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_rows,
+                   int box_cols);
+
 // Opts the kernel into the large dynamic shared memory carve-out (once per device).
 template <class Kernel>
 int ensure_smem_attr(Kernel kernel, std::atomic<uint64_t>& done_mask, int bytes) {
@@ -145,6 +149,46 @@ int max_pair_clusters(Kernel kernel, std::atomic<int>* cache, int smem_bytes, in
   FRX_REQUIRE(n >= 1, FRX_ERR_CUDA, "no 2-CTA cluster of the GEMM kernel fits on this device");
   if (dev < 64) cache[dev].store(n, std::memory_order_relaxed);
   *out = n;
+  return FRX_OK;
+}
+
+// Launches the pair kernel on signed 8-bit operands: D[m, n] = sum_k a[m, k] b[n, k] in int32, both
+// row-major [extent, K] with 16-byte aligned bases and row strides that are multiples of 16.
+template <class Epi>
+int launch_gemm_i8(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int64_t M, int64_t N, int64_t K,
+                   int group_m, const typename Epi::Params& ep, int* status, cudaStream_t stream) {
+  using Cfg = PairCfg<1>;
+  CUtensorMap tm_a, tm_b;
+  int rc = encode_8bit_2d(&tm_a, a, M, K, ld_a, kBM, 128);
+  if (rc) return rc;
+  rc = encode_8bit_2d(&tm_b, b, N, K, ld_b, 128, 128);
+  if (rc) return rc;
+  TileSched sched;
+  sched.num_m = static_cast<int>((M + 255) / 256);
+  sched.num_n = static_cast<int>((N + 255) / 256);
+  sched.n256 = sched.num_n;
+  sched.f16 = 0;
+  sched.stall_kb = -1;
+  sched.wait_limit_ns = kWaitLimitNs;
+  sched.group = group_m < 1 ? 1 : (group_m > sched.num_m ? sched.num_m : group_m);
+  const long long tiles = static_cast<long long>(sched.num_m) * sched.num_n;
+  FRX_REQUIRE(tiles < (1ll << 31), FRX_ERR_INVALID_ARG, "problem too large: %lld output tiles", tiles);
+  sched.num_tiles = static_cast<int>(tiles);
+  const int num_k_blocks = static_cast<int>((K + 2 * Cfg::kStageK - 1) / (2 * Cfg::kStageK));
+  static std::atomic<uint64_t> attr_done{0};
+  static std::atomic<int> clusters_cache[64];
+  auto kernel = gemm_tcgen05_pair_kernel<false, false, 1, Epi, true>;
+  constexpr int smem = gemm_smem_bytes(Cfg::kStages * Cfg::kStageBytes, Epi::kSmemBytes);
+  static_assert(smem <= 232448, "shared memory budget exceeded");
+  rc = ensure_smem_attr(kernel, attr_done, smem);
+  if (rc) return rc;
+  int clusters = 0;
+  rc = max_pair_clusters(kernel, clusters_cache, smem, &clusters);
+  if (rc) return rc;
+  const long long pairs = tiles < clusters ? tiles : clusters;
+  kernel<<<static_cast<unsigned>(2 * pairs), kGemmThreads, smem, stream>>>(tm_a, tm_b, sched, num_k_blocks, ep,
+                                                                           status);
+  FRX_CUDA_CHECK(cudaGetLastError());
   return FRX_OK;
 }
 

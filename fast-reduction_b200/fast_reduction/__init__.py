@@ -14,6 +14,10 @@ __all__ = [
     "gemm_megakernel_fast",
     "vocab_parallel_ce_entropy",
     "vocab_parallel_megakernel",
+    "quantize_int8",
+    "int8_linear",
+    "int8_ce_entropy",
+    "verify_drafts",
 ]
 
 _GEMM_KERNEL_NAMES = {
@@ -23,6 +27,7 @@ _GEMM_KERNEL_NAMES = {
     "gemm_fused_ce_entropy_fast",
     "gemm_megakernel_fast",
 }
+_INT8_HEAD_NAMES = {"quantize_int8", "int8_linear", "int8_ce_entropy"}
 _VOCAB_PARALLEL_NAMES = {"vocab_parallel_ce_entropy", "vocab_parallel_megakernel"}
 
 
@@ -35,4 +40,12 @@ def __getattr__(name):
         from fast_reduction import vocab_parallel
 
         return getattr(vocab_parallel, name)
+    if name in _INT8_HEAD_NAMES:
+        from fast_reduction import int8_head
+
+        return getattr(int8_head, name)
+    if name == "verify_drafts":
+        from fast_reduction import draft_verify
+
+        return draft_verify.verify_drafts
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -44,6 +44,10 @@ FRX_STATUS_TIMEOUT_EPILOGUE = 4
 FRX_STATUS_BAD_TARGET = 8
 FRX_STATUS_DRAIN_TIMEOUT = 16
 FRX_STATUS_CHECK_FAILED = 32
+FRX_STATUS_BAD_OFFSETS = 64
+
+FRX_I8_MAX_K = 131072  # longest row of 8-bit codes whose products cannot overflow an int32 sum
+FRX_VERIFY_CHUNK = 2048  # columns per workspace entry of frx_verify_drafts
 
 _STATUS_NAMES = {
     FRX_STATUS_TIMEOUT_PRODUCER: "TMA producer wait timed out",
@@ -52,6 +56,7 @@ _STATUS_NAMES = {
     FRX_STATUS_BAD_TARGET: "target id outside [0, vocab_size) and not ignore_index",
     FRX_STATUS_DRAIN_TIMEOUT: "in-flight copies did not drain after an abort",
     FRX_STATUS_CHECK_FAILED: "a device-side invariant check of the checked build failed",
+    FRX_STATUS_BAD_OFFSETS: "draft offsets that do not start at 0, decrease or pass the number of drafts",
 }
 
 # Every exported symbol with its ctypes signature: (restype, argtypes).
@@ -86,6 +91,16 @@ SIGNATURES: dict[str, tuple] = {
     "frx_test_stalled_fwd": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I32, _I64, _P, _P]),
     "frx_loss_sum": (_I32, [_P, _P, _I64, _F32, _F32, _P, _P]),
     "frx_scale_inplace": (_I32, [_P, _I32, _I64, _P, _P]),
+    "frx_quantize_i8": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "frx_gemm_i8": (_I32, [_P, _I64, _P, _P, _I64, _P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P, _P]),
+    "frx_fwd_partials_i8": (
+        _I32,
+        [_P, _I64, _P, _P, _I64, _P, _P, _I32, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _P],
+    ),
+    "frx_verify_drafts": (
+        _I32,
+        [_P, _I32, _I64, _P, _P, _P, _P, _P, _I32, _I64, _P, _F32, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _P],
+    ),
     "frx_check_range": (_I32, [_P, _I64]),
     "frx_clock_probe": (_I32, [_P, _I32, _P]),
 }

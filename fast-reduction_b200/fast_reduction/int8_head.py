@@ -1,0 +1,191 @@
+"""The vocabulary head in 8-bit integers: hidden states quantised per token, a weight quantised per
+vocabulary row, products on the int8 tensor cores.
+
+    codes, scale = quantize_int8(weight)                               once
+    logits = int8_linear(hidden, codes, scale)                         serving: logits for the sampler
+    ce, entropy, log_probs = int8_ce_entropy(hidden, codes, scale, target)
+                                                                       scoring: no logits in HBM
+
+Quantisation is symmetric: scale_r = max |x_r| / 127 (fp32), code = the integer nearest to x / scale_r.
+The sums of code products are exact (int32); scales and bias are applied in fp32 and each output is
+rounded once. Nothing here is differentiable: the results carry no gradient, and inputs that require one
+are refused while gradients are enabled.
+
+No counterpart in the reference, whose head is bf16 / fp16 / fp32 (fast_reduction/gemm_kernel.py:276-356);
+int8_ce_entropy returns what its gemm_fused_ce_entropy does.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _native as nat
+from . import gemm_kernel as gk
+from . import ops
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _no_grad_inputs(*tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("the int8 head has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _codes_like(rows: int, cols: int, device: torch.device) -> Tensor:
+    """Uninitialised [rows, cols] int8 codes whose rows start on 16-byte boundaries."""
+    return torch.empty(rows, ops.round_up(max(cols, 1), 16), device=device, dtype=torch.int8)[:, :cols]
+
+
+def _aligned_codes(codes: Tensor) -> Tensor:
+    """`codes` itself when its rows start on 16-byte boundaries, else a copy laid out that way."""
+    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= codes.shape[1] \
+            and codes.data_ptr() % 16 == 0:
+        return codes
+    out = _codes_like(codes.shape[0], codes.shape[1], codes.device)
+    out.copy_(codes)
+    return out
+
+
+def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """8-bit codes of the rows of ``x`` [..., K] (bf16, fp16 or fp32): (codes int8 [..., K], scale fp32 [...])
+    with x ~ codes * scale[..., None]. scale = max |row| / 127; each code is the integer nearest to x / scale,
+    ties to even. A row with a NaN or an infinity gets scale NaN and codes 0 (what is computed from it is
+    NaN); a row whose scale would be below 2^-120 gets scale 0 and codes 0.
+
+    For 2-D ``x`` the codes are a view of rows padded to a multiple of 16 bytes, the layout int8_linear
+    reads in place."""
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"quantize_int8 takes bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("quantize_int8 needs at least one dimension")
+    _no_grad_inputs(x)
+    ops._require_cuda(x)
+    codes, scale = _quantize_2d(x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(),
+                                                                                         x.shape[-1]))
+    return codes if x.dim() == 2 else codes.reshape(x.shape), scale.view(x.shape[:-1])
+
+
+def _quantize_2d(x: Tensor) -> Tuple[Tensor, Tensor]:
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    codes = _codes_like(x.shape[0], x.shape[1], x.device)
+    scale = torch.empty(x.shape[0], device=x.device, dtype=torch.float32)
+    ops.quantize_i8(x, codes, scale)
+    return codes, scale
+
+
+def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
+             hidden_scale: Optional[Tensor]):
+    """Checked operands: (batch shape, hidden codes [M, K], hidden scale [M], weight codes, weight scale, bias)."""
+    if weight_codes.dim() != 2 or weight_codes.dtype != torch.int8:
+        raise TypeError(f"weight_codes must be int8 [V, H], got {weight_codes.dtype} {tuple(weight_codes.shape)}")
+    V, H = weight_codes.shape
+    if V < 1 or H < 1:
+        raise ValueError(f"weight_codes must not be empty, got {tuple(weight_codes.shape)}")
+    if H > nat.FRX_I8_MAX_K:
+        raise NotImplementedError(f"hidden size {H} > {nat.FRX_I8_MAX_K} could overflow the int32 sums")
+    if hidden.dim() < 1 or hidden.shape[-1] != H:
+        raise ValueError(f"hidden size mismatch: hidden {tuple(hidden.shape)} vs weight_codes {tuple(weight_codes.shape)}")
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (V,):
+        raise ValueError(f"weight_scale must be float32 [{V}], got {weight_scale.dtype} {tuple(weight_scale.shape)}")
+    if bias is not None:
+        if bias.dtype not in _FLOATS or bias.shape != (V,):
+            raise ValueError(f"bias must be bfloat16, float16 or float32 [{V}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    batch_shape = hidden.shape[:-1]
+    if hidden.dtype == torch.int8:
+        if hidden_scale is None:
+            raise ValueError("int8 hidden states need hidden_scale (one float32 per token)")
+        if hidden_scale.dtype != torch.float32 or hidden_scale.shape != batch_shape:
+            raise ValueError(f"hidden_scale must be float32 {tuple(batch_shape)}, got {hidden_scale.dtype} "
+                             f"{tuple(hidden_scale.shape)}")
+    elif hidden.dtype not in _FLOATS:
+        raise TypeError(f"hidden must be bfloat16, float16, float32 or int8, got {hidden.dtype}")
+    elif hidden_scale is not None:
+        raise ValueError("hidden_scale goes with int8 hidden states; floating-point ones are quantised here")
+    _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
+    ops._require_cuda(hidden, weight_codes, weight_scale, bias, hidden_scale)
+    x = hidden.reshape(-1, H)
+    if hidden.dtype == torch.int8:
+        x, x_scale = _aligned_codes(x), hidden_scale.reshape(-1).contiguous()
+    else:
+        x, x_scale = _quantize_2d(x)
+    return batch_shape, x, x_scale, _aligned_codes(weight_codes), weight_scale.contiguous(), bias
+
+
+def int8_linear(
+    hidden: Tensor,
+    weight_codes: Tensor,
+    weight_scale: Tensor,
+    bias: Optional[Tensor] = None,
+    *,
+    hidden_scale: Optional[Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+    out: Optional[Tensor] = None,
+) -> Tensor:
+    """Logits [..., V] = hidden @ dequantised(weight).T (+ bias) with hidden quantised per token.
+
+    hidden        [..., H] bf16 / fp16 / fp32 (quantised here), or int8 codes with ``hidden_scale`` [...]
+    weight_codes  [V, H] int8 and weight_scale [V] fp32, e.g. from quantize_int8(weight). Codes whose rows do
+                  not start on 16-byte boundaries are copied on every call; quantize_int8 lays them out so
+    bias          optional [V] bf16 / fp16 / fp32
+    out_dtype     bf16, fp16 or fp32; default: hidden's type, bf16 for int8 hidden
+    out           optional [rows, V] output (any row stride, unit column stride), instead of a new tensor
+    """
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else (torch.bfloat16 if hidden.dtype == torch.int8 else hidden.dtype)
+    if out_dtype not in _FLOATS:
+        raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    V = weight_codes.shape[0]
+    rows = hidden.shape[:-1].numel()
+    if out is not None and (out.dtype != out_dtype or out.shape != (rows, V) or (V > 1 and out.stride(1) != 1)
+                            or (rows > 1 and out.stride(0) < V)):
+        raise ValueError(f"out must be {out_dtype} [{rows}, {V}] with unit column stride and rows that do not overlap, "
+                         f"got {out.dtype} {tuple(out.shape)} stride {out.stride()}")
+    batch_shape, x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
+    y = torch.empty(rows, V, device=x.device, dtype=out_dtype) if out is None else out
+    ops.gemm_i8(x, x_scale, w, w_scale, y, bias=bias)
+    return y.view(*batch_shape, V) if out is None else out
+
+
+def int8_ce_entropy(
+    hidden: Tensor,
+    weight_codes: Tensor,
+    weight_scale: Tensor,
+    target: Tensor,
+    bias: Optional[Tensor] = None,
+    chunk_size: int = 4096,
+    ignore_index: int = gk.IGNORE_INDEX,
+    *,
+    hidden_scale: Optional[Tensor] = None,
+) -> Tuple[Tensor, Tensor, Tensor]:
+    """(ce_loss, entropy, log_probs), each fp32 and shaped like ``hidden.shape[:-1]``, of the logits
+    int8_linear would give in fp32, which never reach HBM. Operands as in int8_linear; target, chunk_size and
+    ignore_index as in gemm_fused_ce_entropy (ignored rows: ce = log_probs = 0, entropy kept; a target
+    outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET)."""
+    batch_shape, x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
+    target = target.reshape(-1)
+    B = x.shape[0]
+    if target.numel() != B:
+        raise ValueError(f"target has {target.numel()} elements, expected {B}")
+    if target.dtype.is_floating_point or target.dtype.is_complex or target.dtype == torch.bool:
+        raise TypeError(f"target must be an integer tensor, got {target.dtype}")
+    target = target.to(torch.int64).contiguous()
+    ops._require_cuda(x, target)
+    ce, ent, logp = (torch.empty(B, device=x.device, dtype=torch.float32) for _ in range(3))
+    chunk = gk._chunk_rows(chunk_size, B)
+    if B:
+        V = w.shape[0]
+        T = ops.n_vocab_tiles(V)
+        chunk = gk._launch_rows(chunk, B, T)
+        partials = torch.empty(T, chunk, 4, device=x.device, dtype=torch.float32)
+        for a in range(0, B, chunk):
+            b = min(a + chunk, B)
+            with ops.phase("frx.int8.chunk"):
+                ops.fwd_partials_i8(x[a:b], x_scale[a:b], w, w_scale, target[a:b], partials, chunk, bias=bias)
+            ops.finalize(partials, T, b - a, chunk, target=target[a:b], vocab_size=V, ignore_index=ignore_index,
+                         ce=ce[a:b], entropy=ent[a:b], log_probs=logp[a:b])
+    return ce.view(batch_shape), ent.view(batch_shape), logp.view(batch_shape)

@@ -471,3 +471,106 @@ def scale_inplace(x: torch.Tensor, scale: torch.Tensor) -> None:
     rc = _launch("scale_inplace", dev, lambda: lib.frx_scale_inplace(
         x.data_ptr(), _OUT_DTYPES[x.dtype], x.numel(), scale.data_ptr(), nat.stream_of(dev)))
     nat.check(rc, "frx_scale_inplace")
+
+
+def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
+    """codes (int8), scale (fp32 per row) <- symmetric 8-bit codes of the rows of x (frx_quantize_i8)."""
+    dev = _require_cuda(x, codes, scale)
+    if x.dtype not in _OUT_DTYPES or codes.dtype != torch.int8 or scale.dtype != torch.float32:
+        raise TypeError("quantize_i8 takes a bfloat16, float16 or float32 matrix, int8 codes and float32 scales")
+    if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
+        raise ValueError("codes must have x's shape and scale one value per row")
+    lib = nat.load()
+    with torch.cuda.device(dev):
+        rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
+            x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
+            scale.data_ptr(), nat.stream_of(dev)))
+    nat.check(rc, "frx_quantize_i8")
+
+
+def _i8_operands(x, x_scale, weight, weight_scale, bias):
+    if x.dtype != torch.int8 or weight.dtype != torch.int8:
+        raise TypeError(f"codes must be int8, got {x.dtype} and {weight.dtype}")
+    ldx, ldw = _row_major(x, "x"), _row_major(weight, "weight")
+    if x.shape[1] != weight.shape[1]:
+        raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
+    for name, t, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
+        if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 [{n}]")
+    if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (weight.shape[0],)
+                             or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous bfloat16, float16 or float32 vector with one value per weight row")
+    return ldx, ldw, 0 if bias is None else _OUT_DTYPES[bias.dtype]
+
+
+def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+            out: torch.Tensor, *, bias: torch.Tensor | None = None) -> None:
+    """out[r, j] <- (x[r] . weight[j]) * x_scale[r] * weight_scale[j] (+ bias[j]) for int8 codes (frx_gemm_i8)."""
+    dev = _require_cuda(x, x_scale, weight, weight_scale, bias, out)
+    ldx, ldw, bdt = _i8_operands(x, x_scale, weight, weight_scale, bias)
+    if out.dtype not in _OUT_DTYPES or out.shape != (x.shape[0], weight.shape[0]):
+        raise ValueError(f"out must be bfloat16, float16 or float32 [{x.shape[0]}, {weight.shape[0]}]")
+    lib = nat.load()
+    with torch.cuda.device(dev):
+        rc = _launch("gemm_i8", dev, lambda: lib.frx_gemm_i8(
+            x.data_ptr(), ldx, x_scale.data_ptr(), weight.data_ptr(), ldw, weight_scale.data_ptr(), nat.ptr(bias), bdt,
+            x.shape[0], weight.shape[0], x.shape[1], out.data_ptr(), max(out.stride(0), out.shape[1]),
+            _OUT_DTYPES[out.dtype], nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    nat.check(rc, "frx_gemm_i8")
+
+
+def fwd_partials_i8(hidden: torch.Tensor, hidden_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                    target: torch.Tensor | None, partials: torch.Tensor, tile_stride: int, vocab_offset: int = 0, *,
+                    bias: torch.Tensor | None = None) -> None:
+    """fwd_partials of the logits gemm_i8 would give (frx_fwd_partials_i8)."""
+    dev = _require_cuda(hidden, hidden_scale, weight, weight_scale, target, partials, bias)
+    ldh, ldw, bdt = _i8_operands(hidden, hidden_scale, weight, weight_scale, bias)
+    rows, vshard = hidden.shape[0], weight.shape[0]
+    if target is not None and (target.dtype != torch.int64 or not target.is_contiguous() or target.numel() < rows):
+        raise ValueError("target must be a contiguous int64 tensor with one id per row")
+    if partials.dtype != torch.float32 or not partials.is_contiguous() or tile_stride < rows or \
+            partials.numel() < 4 * ((n_vocab_tiles(vshard) - 1) * tile_stride + rows):
+        raise ValueError("partials must be contiguous float32 covering every tile of the launch")
+    lib = nat.load()
+    with torch.cuda.device(dev):
+        rc = _launch("fwd_partials_i8", dev, lambda: lib.frx_fwd_partials_i8(
+            hidden.data_ptr(), ldh, hidden_scale.data_ptr(), weight.data_ptr(), ldw, weight_scale.data_ptr(),
+            nat.ptr(bias), bdt, nat.ptr(target), rows, vshard, hidden.shape[1], vocab_offset, partials.data_ptr(),
+            tile_stride, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    nat.check(rc, "frx_fwd_partials_i8")
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor, uniforms: torch.Tensor,
+                  final_uniforms: torch.Tensor, draft_probs: torch.Tensor | None, temperature: torch.Tensor | None,
+                  temperature_all: float, workspace: torch.Tensor, accepted: torch.Tensor, tokens: torch.Tensor,
+                  log_probs: torch.Tensor) -> None:
+    """accepted, tokens, log_probs <- the outcome of drafted tokens against target logits (frx_verify_drafts)."""
+    dev = _require_cuda(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature, workspace,
+                        accepted, tokens, log_probs)
+    n, batch = drafts.numel(), cu_drafts.numel() - 1
+    if logits.dtype not in _LOGITS_DTYPES or (draft_probs is not None and draft_probs.dtype not in _LOGITS_DTYPES):
+        raise TypeError("logits and draft_probs must be bfloat16, float16 or float32")
+    ldl = max(_row_major(logits, "logits"), logits.shape[1])
+    vocab = logits.shape[1]
+    ldq = 0 if draft_probs is None else max(_row_major(draft_probs, "draft_probs"), vocab)
+    if logits.shape[0] != n + batch or (draft_probs is not None and draft_probs.shape != (n, vocab)):
+        raise ValueError("logits must have one row per draft and sequence, draft_probs one per draft")
+    for name, t, num, dt in (("drafts", drafts, n, torch.int64), ("cu_drafts", cu_drafts, batch + 1, torch.int64),
+                             ("uniforms", uniforms, n, torch.float32),
+                             ("final_uniforms", final_uniforms, batch, torch.float32),
+                             ("temperature", temperature, batch, torch.float32),
+                             ("accepted", accepted, batch, torch.int64), ("tokens", tokens, n + batch, torch.int64),
+                             ("log_probs", log_probs, n + batch, torch.float32)):
+        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() != num):
+            raise ValueError(f"{name} must be contiguous {dt} with {num} elements")
+    if workspace.dtype != torch.float32 or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous float32")
+    lib = nat.load()
+    with torch.cuda.device(dev):
+        rc = _launch("verify_drafts", dev, lambda: lib.frx_verify_drafts(
+            logits.data_ptr(), _LOGITS_DTYPES[logits.dtype], ldl, drafts.data_ptr(), cu_drafts.data_ptr(),
+            uniforms.data_ptr(), final_uniforms.data_ptr(), nat.ptr(draft_probs),
+            0 if draft_probs is None else _LOGITS_DTYPES[draft_probs.dtype], ldq, nat.ptr(temperature),
+            temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
+            tokens.data_ptr(), log_probs.data_ptr(), nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    nat.check(rc, "frx_verify_drafts")

@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define FRX_ABI_VERSION 4
+#define FRX_ABI_VERSION 5
 
 #define FRX_OK 0
 #define FRX_ERR_INVALID_ARG 1
@@ -72,6 +72,7 @@ extern "C" {
 #define FRX_STATUS_BAD_TARGET 8
 #define FRX_STATUS_DRAIN_TIMEOUT 16
 #define FRX_STATUS_CHECK_FAILED 32 /* a device-side invariant check of a checked build failed */
+#define FRX_STATUS_BAD_OFFSETS 64  /* draft offsets that do not start at 0, decrease or pass the drafts */
 
 /* ABI version of the loaded library (FRX_ABI_VERSION it was built with). */
 FRX_API int frx_abi_version(void);
@@ -295,6 +296,71 @@ FRX_API int frx_loss_sum(const float* ce, const float* entropy, int64_t rows, fl
  * gradients.
  */
 FRX_API int frx_scale_inplace(void* x, int dtype, int64_t n, const float* scale, void* stream);
+
+/*
+ * Symmetric 8-bit codes of the rows of x [rows, cols] (dtype BF16, F16 or F32, row stride ld_x):
+ *   scale[r] = fl32(max_c |x[r, c]| / 127),  codes[r, c] = the integer nearest to x[r, c] / scale[r], ties to even
+ * (|code| <= 127). A row with a NaN or an infinity gets scale NaN and codes 0, so what is computed from
+ * it is NaN; a row whose scale would be below 2^-120 gets scale 0 and codes 0. Columns [cols, ld_codes)
+ * of `codes` are left as they were. For frx_gemm_i8, codes need a 16-byte aligned base and ld_codes a
+ * multiple of 16. No counterpart in the reference.
+ */
+FRX_API int frx_quantize_i8(const void* x, int dtype, int64_t ld_x, int64_t rows, int64_t cols, void* codes,
+                            int64_t ld_codes, float* scale, void* stream);
+
+/*
+ * out[r, j] = (sum_c x[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]) for signed 8-bit codes
+ * x [rows, k] and weight [cols, k] (row strides ld_x, ld_weight: multiples of 16, bases 16-byte aligned):
+ * exact int32 sums (k <= 131072, codes within +-127), scaled in fp32 and rounded once to out_dtype (BF16,
+ * F16 or F32; any ld_out >= cols and any alignment of the element type). bias (bias_dtype BF16, F16 or
+ * F32) may be NULL. No counterpart in the reference.
+ */
+FRX_API int frx_gemm_i8(const void* x, int64_t ld_x, const float* x_scale, const void* weight, int64_t ld_weight,
+                        const float* weight_scale, const void* bias, int bias_dtype, int64_t rows, int64_t cols,
+                        int64_t k, void* out, int64_t ld_out, int out_dtype, int* status, void* stream);
+
+/*
+ * frx_fwd_partials on 8-bit codes: the logits of frx_gemm_i8, reduced to the same (m, s, u, zt) partials by
+ * the epilogue; frx_finalize merges them. Operands as in frx_gemm_i8, the rest as in frx_fwd_partials.
+ * No counterpart in the reference.
+ */
+FRX_API int frx_fwd_partials_i8(const void* hidden, int64_t ld_hidden, const float* hidden_scale, const void* weight,
+                                int64_t ld_weight, const float* weight_scale, const void* bias, int bias_dtype,
+                                const int64_t* target, int64_t rows, int64_t vocab_shard, int64_t hidden_dim,
+                                int64_t vocab_offset, float* partials, int64_t tile_stride, int* status, void* stream);
+
+/*
+ * Verifies drafted tokens against the target model's logits (speculative sampling) from given random
+ * numbers. Sequence b has drafts [cu_drafts[b], cu_drafts[b + 1]) (n of them, possibly none) and n + 1
+ * rows of logits from row cu_drafts[b] + b. With p_i = softmax(row i / T_b), draft i is accepted while
+ *   uniforms[draft] * draft_probs[draft, d] < p_i(d)          (draft_probs NULL: 1 * uniform < p_i(d)),
+ * and the sequence emits its accepted drafts and one more token, drawn as the first j with w_j > 0 and
+ * sum_{k<=j} w_k > final_uniforms[b] * sum_k w_k, where w = max(p - q, 0) at the rejected draft's row (NULL:
+ * p without the rejected token; p itself when nothing is left), or p of the last row after full acceptance.
+ * Decisions are taken in 64 bits. T < 1e-6 (or NaN) is greedy: a draft must equal its row's argmax
+ * (lowest index of a tie) and the argmax is emitted. T above 1e6 counts as 1e6. NaN logits count as -inf,
+ * +inf as the largest float, negative or NaN draft probabilities as 0; a row with nothing left to draw emits
+ * -1 with log-probability -inf.
+ *   logits       [n_drafts + batch, vocab] (dtype BF16, F16 or F32, row stride ld_logits)
+ *   drafts       [n_drafts] token ids; one outside [0, vocab) is rejected (FRX_STATUS_BAD_TARGET)
+ *   cu_drafts    [batch + 1] non-decreasing from 0; cu_drafts[batch] may be below n_drafts (a padded batch:
+ *                rows behind the last sequence's are not read). Offsets are clamped into [0, n_drafts];
+ *                bad ones set FRX_STATUS_BAD_OFFSETS
+ *   draft_probs  [n_drafts, vocab] (BF16, F16 or F32, row stride ld_draft_probs) or NULL
+ *   temperature  [batch] or NULL (then temperature_all)
+ *   workspace    at least 4 * (n_drafts + batch) * ceil(vocab / 2048) floats, 16-byte aligned; its contents
+ *                need not be kept between calls, and calls that overlap need one each
+ *   accepted     [batch] number of accepted drafts
+ *   tokens, log_probs  [n_drafts + batch], at the rows of the logits: the emitted tokens and their log p_i
+ *                (greedy: at T = 1); -1 and 0 where nothing is emitted, rows behind the last sequence's too
+ * No counterpart in the reference.
+ */
+FRX_API int frx_verify_drafts(const void* logits, int dtype, int64_t ld_logits, const int64_t* drafts,
+                              const int64_t* cu_drafts, const float* uniforms, const float* final_uniforms,
+                              const void* draft_probs, int draft_probs_dtype, int64_t ld_draft_probs,
+                              const float* temperature, float temperature_all, int64_t batch, int64_t n_drafts,
+                              int64_t vocab, float* workspace, int64_t workspace_floats, int64_t* accepted,
+                              int64_t* tokens, float* log_probs, int* status, void* stream);
 
 /*
  * FRX_OK when the `bytes` bytes from `ptr` lie inside one device allocation (cuMemGetAddressRange),

@@ -31,6 +31,10 @@ ARGTYPES = {
     "frx_fwd_ce_entropy_noalloc": [P, I64, P, I64, P, I64, I64, I64, I64, P, P, P, P, P, P],
     "frx_gemm_dhidden_multicast": [P, I64, P, I64, I32, P, I64, I64, I64, I64, P, P],
     "frx_test_stalled_fwd": [P, I64, P, I64, P, I64, I64, I64, P, I64, I32, I64, P, P],
+    "frx_quantize_i8": [P, I32, I64, I64, I64, P, I64, P, P],
+    "frx_gemm_i8": [P, I64, P, P, I64, P, P, I32, I64, I64, I64, P, I64, I32, P, P],
+    "frx_fwd_partials_i8": [P, I64, P, P, I64, P, P, I32, P, I64, I64, I64, I64, P, I64, P, P],
+    "frx_verify_drafts": [P, I32, I64, P, P, P, P, P, I32, I64, P, F32, I64, I64, I64, P, I64, P, P, P, P, P],
     "frx_check_range": [P, I64],
     "frx_clock_probe": [P, I32, P],
     "frx_abi_version": [],
@@ -173,3 +177,40 @@ def fwd_ce_entropy_noalloc(A, W, target, ce, entropy, lse, log_probs, ignore_ind
     _check(_lib.frx_fwd_ce_entropy_noalloc(A.data_ptr(), A.stride(0), W.data_ptr(), W.stride(0), target.data_ptr(),
                                            M, V, K, ignore_index, ce.data_ptr(), entropy.data_ptr(), _ptr(lse),
                                            _ptr(log_probs), None, _stream(A)))
+
+
+def quantize_i8(X, codes, scale):
+    """8-bit codes and one scale per row of a float matrix (no counterpart in the reference)."""
+    M, K = X.shape
+    _check(_lib.frx_quantize_i8(X.data_ptr(), FRX_DTYPE[X.dtype], X.stride(0), M, K, codes.data_ptr(),
+                                codes.stride(0), scale.data_ptr(), _stream(X)))
+
+
+def gemm_i8(Xq, x_scale, Wq, w_scale, out, *, bias=None):
+    """Logits of 8-bit codes (row strides multiples of 16) with scales per row of each operand."""
+    M, K = Xq.shape
+    V = Wq.shape[0]
+    _check(_lib.frx_gemm_i8(Xq.data_ptr(), Xq.stride(0), x_scale.data_ptr(), Wq.data_ptr(), Wq.stride(0),
+                            w_scale.data_ptr(), _ptr(bias), 0 if bias is None else FRX_DTYPE[bias.dtype], M, V, K,
+                            out.data_ptr(), out.stride(0), FRX_DTYPE[out.dtype], None, _stream(Xq)))
+
+
+def fwd_partials_i8(Aq, a_scale, Wq, w_scale, target, partials, *, bias=None, vocab_offset=0):
+    """fwd_partials on 8-bit codes; partials: fp32 [ceil(V / 256), M, 4]."""
+    M, K = Aq.shape
+    V = Wq.shape[0]
+    _check(_lib.frx_fwd_partials_i8(Aq.data_ptr(), Aq.stride(0), a_scale.data_ptr(), Wq.data_ptr(), Wq.stride(0),
+                                    w_scale.data_ptr(), _ptr(bias), 0 if bias is None else FRX_DTYPE[bias.dtype],
+                                    _ptr(target), M, V, K, vocab_offset, partials.data_ptr(), M, None, _stream(Aq)))
+
+
+def verify_drafts(L, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature, workspace, accepted, tokens,
+                  log_probs):
+    """Speculative-sampling verification of drafted tokens against the logits L [N + B, V]."""
+    B, N, V = final_uniforms.shape[0], drafts.shape[0], L.shape[1]
+    _check(_lib.frx_verify_drafts(L.data_ptr(), FRX_DTYPE[L.dtype], L.stride(0), drafts.data_ptr(),
+                                  cu_drafts.data_ptr(), uniforms.data_ptr(), final_uniforms.data_ptr(),
+                                  _ptr(draft_probs), 0 if draft_probs is None else FRX_DTYPE[draft_probs.dtype],
+                                  0 if draft_probs is None else draft_probs.stride(0), temperature.data_ptr(), 1.0, B,
+                                  N, V, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
+                                  tokens.data_ptr(), log_probs.data_ptr(), None, _stream(L)))

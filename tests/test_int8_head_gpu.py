@@ -1,0 +1,291 @@
+"""GPU: the 8-bit head (quantize_int8, int8_linear, int8_ce_entropy) against plain 64-bit computations.
+
+Tolerances. Codes and scales are compared exactly: the scale is one fp32 division, a code the integer
+nearest to the real quotient. A logit is an exact integer sum turned into fp32 (half a step, 2^-24), times two
+scales (2^-24 each), plus a bias (2^-24 of the sum), rounded to the output type (half a step of it):
+    |y - y64| <= finfo(out).eps / 2 * |y64| + 4 * 2^-24 * (|product| + |bias|) * (1 + 2^-8) + smallest subnormal.
+For the reductions, with L = max |z| of the row and D = max z - min z: a logit is off by at most 4 * 2^-24 * L',
+L' = |product| + |bias|; a base-2 exponential by 2^-22 relative plus its argument's rounding (2 * 2^-24 * D); sums
+of 128 terms in fp32 in each tile half (128 * 2^-24), then at most 512 merges of 2^-22 each:
+    rel = 2^-22 + 2^-23 * D + 2^-17 + 2^-13      (of S; of U the same, times its terms |z - m| <= D)
+    |ce - ce64| <= rel + 8 * 2^-24 * L' + 2^-23 * |ce64|,   |H - H64| <= rel * (2 + 2 * D) + 8 * 2^-24 * L' * (1 + D).
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+FLOATS = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture(autouse=True)
+def _status_clean():
+    from fast_reduction import _native as nat
+
+    nat.read_status(torch.device(DEV))
+    yield
+    torch.cuda.synchronize()
+    nat.raise_on_status(torch.device(DEV))
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def ref_quantize(x):
+    """Codes (float64 integers) and scales (float32) by definition."""
+    x64 = x.double()
+    amax = x.float().abs().amax(-1) if x.shape[-1] else x.new_zeros(x.shape[:-1], dtype=torch.float32)
+    scale = (amax.double() / 127).float()  # 24-bit operands: rounding the 64-bit quotient once is the fp32 division
+    bad = ~torch.isfinite(amax)
+    scale = torch.where(scale < 2.0**-120, torch.zeros_like(scale), scale)
+    live = (scale > 0) & ~bad
+    scale = torch.where(bad, torch.full_like(scale, float("nan")), scale)
+    codes = torch.round(x64 / torch.where(live, scale, torch.ones_like(scale)).double()[..., None])
+    return torch.where(live[..., None], codes, torch.zeros_like(codes)), scale
+
+
+def ref_logits(codes, scale, wcodes, wscale, bias):
+    prod = (codes.double() @ wcodes.double().t()) * scale.double()[:, None] * wscale.double()[None, :]
+    b = torch.zeros(wcodes.shape[0], device=DEV, dtype=torch.float64) if bias is None else bias.double()
+    return prod + b, prod.abs() + b.abs()
+
+
+def assert_logits(y, z, mag):
+    fi = torch.finfo(y.dtype)
+    tol = fi.eps / 2 * z.abs() + 4 * 2.0**-24 * mag * (1 + 2.0**-8) + fi.smallest_normal * fi.eps
+    bad = ~((y.double() - z).abs() <= tol) & ~(torch.isnan(z) & torch.isnan(y))
+    assert not bad.any(), (int(bad.sum()), y[bad][:4], z[bad][:4])
+
+
+def make(rows, k, v, dtype, seed, bias=None):
+    from fast_reduction import quantize_int8
+
+    g = _gen(seed)
+    x = torch.randn(rows, k, device=DEV, generator=g).to(dtype)
+    codes, scale = quantize_int8((torch.randn(v, k, device=DEV, generator=g) * k**-0.5))
+    b = None if bias is None else torch.randn(v, device=DEV, generator=g).to(bias)
+    return x, codes, scale, b
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 8), (3, 17), (2, 16), (5, 1000), (1, 4096), (1300, 520), (257, 4096),
+                                       (2, 20001), (1201, 72), (1, 131072)])
+def test_quantize_matches_definition(dtype, rows, cols):
+    from fast_reduction import quantize_int8
+
+    x = (torch.randn(rows, cols, device=DEV, generator=_gen(rows + cols)) * 3).to(dtype)
+    codes, scale = quantize_int8(x)
+    c, s = ref_quantize(x)
+    assert codes.dtype == torch.int8 and codes.stride(0) % 16 == 0
+    assert torch.equal(scale, s)
+    assert torch.equal(codes.double(), c)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantize_halves_and_extreme_rows(dtype):
+    from fast_reduction import quantize_int8
+
+    k = 512
+    x = torch.randn(12, k, device=DEV, generator=_gen(1))
+    big = torch.finfo(dtype).max
+    x[0] = 0
+    x[1, 3] = float("inf")
+    x[2, 4] = float("nan")
+    x[3, 5] = -float("inf")
+    # every quotient a half or next to one: the maximum is 127, so the scale is 1
+    x[4] = (torch.arange(k, device=DEV) % 127).float() + 0.5
+    x[4, 0] = 127
+    x[5] = -x[4]
+    x[6] = torch.where(torch.arange(k, device=DEV) % 2 == 0, 4.0, 2.0)  # max and half of it
+    x[7] = x[7].clamp(-1, 1) * 1e-30  # subnormal or zero in fp16
+    x[8] = x[8].clamp(-1, 1) * 1e-38
+    x[9] = x[9].clamp(-1, 1)
+    x = x.to(dtype)
+    x[9, 7] = big
+    x[10] = big
+    x[11] = -big
+    codes, scale = quantize_int8(x)
+    c, s = ref_quantize(x)
+    assert torch.equal(scale.isnan(), s.isnan()) and torch.equal(scale.nan_to_num(-1), s.nan_to_num(-1))
+    assert torch.equal(codes.double(), c)
+    assert s[[1, 2, 3]].isnan().all() and s[0] == 0
+
+
+def test_quantize_strided_and_many_dimensions():
+    from fast_reduction import quantize_int8
+
+    base = torch.randn(40, 131, device=DEV, generator=_gen(2)).to(torch.bfloat16)
+    for x in (base[:, 1:130], base[::3], base[:, ::2], base.t(), base.view(5, 8, 131), base[0]):
+        codes, scale = quantize_int8(x)
+        c, s = ref_quantize(x)
+        assert codes.shape == x.shape and torch.equal(codes.double(), c) and torch.equal(scale, s)
+    for shape in ((0, 5), (3, 0), (2, 0, 4), (0,)):
+        codes, scale = quantize_int8(torch.empty(shape, device=DEV))
+        assert codes.shape == shape and scale.shape == shape[:-1] and (scale == 0).all()
+
+
+@pytest.mark.parametrize("dtype,out,bias", [(torch.bfloat16, torch.bfloat16, None),
+                                            (torch.float16, torch.float32, torch.float16),
+                                            (torch.float32, torch.float16, torch.float32),
+                                            (torch.bfloat16, torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("rows,k,v", [(1, 16, 1), (1, 1, 5), (1, 1024, 3001), (2, 4096, 640), (7, 100, 129), (16, 256, 256),
+                                      (17, 1000, 127), (37, 1000, 3001), (64, 4096, 1280), (100, 520, 333),
+                                      (128, 128, 128), (129, 129, 515), (256, 384, 257), (300, 4096, 1000),
+                                      (515, 65, 700)])
+def test_linear_matches_64_bits(dtype, out, bias, rows, k, v):
+    from fast_reduction import int8_linear
+
+    x, w, ws, b = make(rows, k, v, dtype, rows * 7 + k + v, bias)
+    y = int8_linear(x, w, ws, bias=b, out_dtype=out)
+    assert y.dtype == out and y.shape == (rows, v)
+    c, s = ref_quantize(x)
+    assert_logits(y, *ref_logits(c, s, w, ws, b))
+    assert torch.equal(y, int8_linear(x, w, ws, bias=b, out_dtype=out))  # deterministic
+
+
+@pytest.mark.parametrize("rows", [1, 30, 400])
+def test_linear_sums_are_exact_at_the_limits(rows):
+    """All codes +-127 over the longest row: the largest sums, which fp32 accumulation could not hold exactly."""
+    from fast_reduction import int8_linear
+
+    k, v = 131072, 200
+    g = _gen(5)
+    x = torch.full((rows, k), 127, device=DEV, dtype=torch.int8)
+    w = torch.full((v, k), 127, device=DEV, dtype=torch.int8)
+    x[:, ::9] = torch.randint(-127, 128, x[:, ::9].shape, device=DEV, generator=g, dtype=torch.int8)
+    w[1::2] *= -1
+    one = torch.ones(rows, device=DEV)
+    y = int8_linear(x, w, torch.ones(v, device=DEV), hidden_scale=one, out_dtype=torch.float32)
+    exact = x.double() @ w.double().t()
+    assert torch.equal(y, exact.float())
+
+
+def test_linear_operand_layouts():
+    from fast_reduction import int8_linear, quantize_int8
+
+    x, w, ws, _ = make(24, 144, 300, torch.bfloat16, 11)
+    y = int8_linear(x, w, ws)
+    assert torch.equal(int8_linear(x.view(2, 3, 4, 144), w, ws), y.view(2, 3, 4, 300))
+    assert torch.equal(int8_linear(x[3], w, ws), y[3])
+    wide = torch.zeros(24, 300, device=DEV, dtype=torch.bfloat16)
+    wide[:, 7:151] = x
+    assert torch.equal(int8_linear(wide[:, 7:151], w, ws), y)
+    assert torch.equal(int8_linear(x.t().contiguous().t(), w, ws), y)
+    # codes that do not start on 16-byte boundaries, and a strided scale
+    odd = torch.zeros(300, 147, device=DEV, dtype=torch.int8)
+    odd[:, 2:146] = w
+    ws2 = torch.stack([ws, ws], 1)[:, 0]
+    assert torch.equal(int8_linear(x, odd[:, 2:146], ws2), y)
+    # int8 hidden states, 8 tokens per group
+    c, s = quantize_int8(x.view(3, 8, 144))
+    assert torch.equal(int8_linear(c, w, ws, hidden_scale=s), y.view(3, 8, 300))
+    # an output with longer rows: the rest of it stays as it was
+    for dt in FLOATS:
+        for off in (0, 1, 5):
+            buf = torch.full((26, 311), 7.0, device=DEV, dtype=dt)
+            got = int8_linear(x, w, ws, out=buf[1:25, off:off + 300])
+            assert got.data_ptr() == buf[1:25, off:].data_ptr()
+            assert torch.equal(got, int8_linear(x, w, ws, out_dtype=dt))
+            rest = buf.clone()
+            rest[1:25, off:off + 300] = 7.0
+            assert (rest == 7.0).all()
+    assert int8_linear(x[:0], w, ws).shape == (0, 300)
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_bad_tokens_and_weights_stay_in_their_row_and_column(rows):
+    from fast_reduction import int8_linear, quantize_int8
+
+    x, _, _, _ = make(rows, 256, 4, torch.float32, 3)
+    wf = torch.randn(300, 256, device=DEV, generator=_gen(8))
+    good = int8_linear(x, *quantize_int8(wf))
+    x2, wf2 = x.clone(), wf.clone()
+    x2[1, 5] = float("nan")
+    wf2[70, 9] = float("inf")
+    wf2[71] = 0
+    y = int8_linear(x2, *quantize_int8(wf2))
+    assert y[1].isnan().all() and y[:, 70].isnan().all()
+    rows = [r for r in range(rows) if r != 1]
+    cols = [c for c in range(300) if c not in (70, 71)]
+    assert torch.equal(y[rows][:, cols], good[rows][:, cols]) and (y[rows, 71] == 0).all()
+
+
+def ref_score(z, mag, t):
+    lse = torch.logsumexp(z, -1)
+    ls = z - lse[:, None]
+    ent = -(ls.exp() * ls).sum(-1)
+    ok = t >= 0
+    ce = torch.where(ok, lse - z.gather(1, t.clamp(min=0)[:, None])[:, 0], torch.zeros_like(lse))
+    big, d = mag.amax(-1), z.amax(-1) - z.amin(-1)
+    rel = 2.0**-22 + 2.0**-23 * d + 2.0**-17 + 2.0**-13
+    return ce, ent, rel + 8 * 2.0**-24 * big + 2.0**-23 * ce.abs(), rel * (2 + 2 * d) + 8 * 2.0**-24 * big * (1 + d)
+
+
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, None), (torch.float16, torch.float16),
+                                        (torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("rows,k,v", [(1, 16, 1), (1, 1024, 3001), (3, 17, 20), (64, 512, 257), (130, 129, 1000),
+                                      (300, 1000, 5000), (517, 256, 32000)])
+def test_score_matches_64_bits(dtype, bias, rows, k, v):
+    from fast_reduction import int8_ce_entropy
+
+    x, w, ws, b = make(rows, k, v, dtype, rows + k + v, bias)
+    x = x * 3
+    t = torch.randint(0, v, (rows,), device=DEV, generator=_gen(4))
+    t[::5] = -100
+    if rows > 2:
+        t[1] = v - 1
+    ce, ent, lp = int8_ce_entropy(x, w, ws, t, bias=b)
+    c, s = ref_quantize(x)
+    z, mag = ref_logits(c, s, w, ws, b)
+    ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, t)
+    assert ((ce.double() - ce_r).abs() <= tol_ce).all()
+    assert ((ent.double() - ent_r).abs() <= tol_ent).all()
+    assert torch.equal(lp, -ce) and (ce[t < 0] == 0).all()
+
+
+def test_score_chunks_shapes_and_int8_hidden():
+    from fast_reduction import int8_ce_entropy, quantize_int8
+
+    x, w, ws, b = make(600, 384, 2001, torch.bfloat16, 21, torch.float32)
+    t = torch.randint(0, 2001, (600,), device=DEV, generator=_gen(6))
+    whole = int8_ce_entropy(x, w, ws, t, bias=b)
+    for chunk in (1, 77, 256, 600):
+        for a, e in zip(int8_ce_entropy(x, w, ws, t, bias=b, chunk_size=chunk), whole):
+            assert torch.equal(a, e)
+    c, s = quantize_int8(x.view(20, 30, 384))
+    for a, e in zip(int8_ce_entropy(c, w, ws, t.view(20, 30).int(), bias=b, hidden_scale=s), whole):
+        assert a.shape == (20, 30) and torch.equal(a.reshape(-1), e)
+    for a in int8_ce_entropy(x[:0], w, ws, t[:0]):
+        assert a.shape == (0,)
+
+
+def test_score_bad_target_sets_status_and_nan():
+    from fast_reduction import _native as nat
+    from fast_reduction import int8_ce_entropy
+
+    x, w, ws, _ = make(8, 64, 300, torch.bfloat16, 2)
+    t = torch.tensor([0, 299, 300, 5, -1, 7, 8, -100], device=DEV)
+    ce, ent, _ = int8_ce_entropy(x, w, ws, t)
+    assert nat.read_status(torch.device(DEV)) == nat.FRX_STATUS_BAD_TARGET
+    assert ce[[2, 4]].isnan().all() and ce[[0, 1, 3, 5, 6, 7]].isfinite().all() and ent.isfinite().all()
+
+
+def test_other_stream_and_two_streams_at_once():
+    from fast_reduction import int8_ce_entropy, int8_linear
+
+    x, w, ws, _ = make(48, 2048, 4000, torch.bfloat16, 31)
+    t = torch.randint(0, 4000, (48,), device=DEV, generator=_gen(6))
+    want = int8_linear(x, w, ws)
+    score = int8_ce_entropy(x, w, ws, t)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((int8_linear(x, w, ws), int8_ce_entropy(x, w, ws, t)))
+    torch.cuda.synchronize()
+    for y, sc in got:
+        assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(sc, score))

@@ -1,0 +1,153 @@
+"""CPU: the 8-bit head and the draft verification refuse bad arguments before any GPU work, in Python and at the
+C entry points (which read nothing through the pointers they are given here)."""
+
+import pytest
+import torch
+
+A, B, C, D = 1 << 20, 1 << 21, 1 << 22, 1 << 23  # aligned addresses that are never read
+
+
+def _lib():
+    from fast_reduction import _native as nat
+
+    return nat, nat.load()
+
+
+def test_quantize_entry_point():
+    nat, lib = _lib()
+    assert lib.frx_quantize_i8(A, 0, 8, -1, 8, B, 16, C, None) == nat.FRX_ERR_INVALID_ARG
+    assert lib.frx_quantize_i8(A, 0, 7, 2, 8, B, 16, C, None) == nat.FRX_ERR_INVALID_ARG  # ld_x < cols
+    assert lib.frx_quantize_i8(A, 0, 8, 2, 8, B, 7, C, None) == nat.FRX_ERR_INVALID_ARG
+    assert lib.frx_quantize_i8(A, 5, 8, 2, 8, B, 16, C, None) == nat.FRX_ERR_INVALID_ARG  # dtype
+    assert lib.frx_quantize_i8(A, 0, 8, 2, 8, None, 16, C, None) == nat.FRX_ERR_INVALID_ARG
+    assert lib.frx_quantize_i8(A, 0, 8, 2, 8, B, 16, None, None) == nat.FRX_ERR_INVALID_ARG
+    assert lib.frx_quantize_i8(None, 0, 8, 0, 8, None, 16, None, None) == nat.FRX_OK
+
+
+@pytest.mark.parametrize("score", [False, True])
+def test_product_entry_points(score):
+    nat, lib = _lib()
+
+    def call(x=A, ld_x=64, xs=B, w=C, ld_w=64, ws=D, bias=None, bdt=0, rows=4, cols=8, k=64, out=A, ld=8, odt=0):
+        if score:
+            return lib.frx_fwd_partials_i8(x, ld_x, xs, w, ld_w, ws, bias, bdt, None, rows, cols, k, 0, out, ld, None,
+                                           None)
+        return lib.frx_gemm_i8(x, ld_x, xs, w, ld_w, ws, bias, bdt, rows, cols, k, out, ld, odt, None, None)
+
+    bad = nat.FRX_ERR_INVALID_ARG
+    assert call(rows=-1) == bad and call(cols=0) == bad and call(k=0) == bad and call(rows=1 << 31) == bad
+    assert call(k=131073, ld_x=131088, ld_w=131088) == nat.FRX_ERR_UNSUPPORTED
+    assert call(x=None) == bad and call(xs=None) == bad and call(w=None) == bad and call(ws=None) == bad
+    assert call(x=A + 8) == bad and call(w=C + 1) == bad and call(ld_x=72) == bad and call(ld_w=48) == bad
+    assert call(bias=A, bdt=7) == bad
+    assert call(out=None) == bad
+    assert call(rows=0) == nat.FRX_OK
+    if score:
+        assert call(ld=3) == bad and call(out=A + 4) == bad  # tile_stride < rows; unaligned partials
+    else:
+        assert call(ld=7) == bad and call(odt=9) == bad
+
+
+def test_verify_entry_point():
+    nat, lib = _lib()
+
+    def call(logits=A, dt=0, ld=100, drafts=B, cu=B, u=B, r=B, q=None, qdt=1, ldq=0, batch=2, n=3, v=100, ws=C,
+             floats=20, acc=D, tok=D, lp=D):
+        return lib.frx_verify_drafts(logits, dt, ld, drafts, cu, u, r, q, qdt, ldq, None, 1.0, batch, n, v, ws, floats,
+                                     acc, tok, lp, None, None)
+
+    bad = nat.FRX_ERR_INVALID_ARG
+    assert call(batch=-1) == bad and call(n=-1) == bad and call(v=0) == bad and call(ld=99) == bad
+    assert call(dt=4) == bad and call(q=A, qdt=8, ldq=100) == bad and call(q=A, ldq=99) == bad
+    for name in ("logits", "drafts", "cu", "u", "r", "ws", "acc", "tok", "lp"):
+        assert call(**{name: None}) == bad, name
+    assert call(floats=19) == bad and b"workspace" in lib.frx_last_error()
+    assert call(ws=C + 4) == bad
+    assert call(batch=0) == bad  # drafts of no sequence
+    assert call(batch=0, n=0) == nat.FRX_OK
+
+
+def test_int8_head_refusals():
+    from fast_reduction import int8_ce_entropy, int8_linear, quantize_int8
+
+    x, w, s = torch.zeros(4, 32), torch.zeros(10, 32, dtype=torch.int8), torch.ones(10)
+    t = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA"):
+        quantize_int8(x)
+    with pytest.raises(TypeError):
+        quantize_int8(torch.zeros(3, 4, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        quantize_int8(torch.zeros(()))
+    for fn in (lambda *a, **k: int8_linear(*a, **k), lambda h, *a, **k: int8_ce_entropy(h, *a, t, **k)):
+        with pytest.raises(ValueError, match="CUDA"):
+            fn(x, w, s)
+        with pytest.raises(TypeError):
+            fn(x, w.float(), s)
+        with pytest.raises(TypeError):
+            fn(x.double(), w, s)
+        with pytest.raises(ValueError, match="mismatch"):
+            fn(x[:, :31], w, s)
+        with pytest.raises(ValueError, match="weight_scale"):
+            fn(x, w, s[:9])
+        with pytest.raises(ValueError, match="weight_scale"):
+            fn(x, w, s.half())
+        with pytest.raises(ValueError, match="bias"):
+            fn(x, w, s, bias=torch.zeros(9))
+        with pytest.raises(ValueError, match="hidden_scale"):
+            fn(x.to(torch.int8), w, s)
+        with pytest.raises(ValueError, match="hidden_scale"):
+            fn(x.to(torch.int8), w, s, hidden_scale=torch.ones(3))
+        with pytest.raises(ValueError, match="hidden_scale"):
+            fn(x, w, s, hidden_scale=torch.ones(4))
+        with pytest.raises(NotImplementedError, match="overflow"):
+            fn(torch.zeros(1, 131073), torch.zeros(2, 131073, dtype=torch.int8), s[:2])
+        with pytest.raises(NotImplementedError, match="gradient"):
+            fn(x.clone().requires_grad_(True), w, s)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            fn(x.clone().requires_grad_(True), w, s)
+        with pytest.raises(ValueError, match="empty"):
+            fn(torch.zeros(4, 0), w[:, :0], s)
+    with pytest.raises(TypeError, match="out_dtype"):
+        int8_linear(x, w, s, out_dtype=torch.float64)
+    for out in (torch.zeros(4, 9), torch.zeros(10, 4).t(), torch.zeros(1, 10).expand(4, 10), torch.zeros(3, 10)):
+        with pytest.raises(ValueError, match="out must"):
+            int8_linear(x, w, s, out=out)
+
+
+def test_verify_refusals():
+    from fast_reduction import verify_drafts
+
+    z, d, cu = torch.zeros(5, 20), torch.zeros(3, dtype=torch.int64), torch.tensor([0, 1, 3])
+    u, r, q = torch.zeros(3), torch.zeros(2), torch.full((3, 20), 0.05)
+
+    def call(**kw):
+        a = dict(target_logits=z, draft_tokens=d, cu_drafts=cu, uniforms=u, final_uniforms=r, draft_probs=q)
+        a.update(kw)
+        return verify_drafts(**a)
+
+    with pytest.raises(ValueError, match="CUDA"):
+        call()
+    with pytest.raises(TypeError):
+        call(draft_tokens=d.float())
+    with pytest.raises(ValueError):
+        call(draft_tokens=d[None])
+    with pytest.raises(TypeError):
+        call(cu_drafts=cu.float())
+    with pytest.raises(ValueError, match="offset"):
+        call(cu_drafts=cu[:0])
+    with pytest.raises(ValueError, match="no sequence"):
+        call(cu_drafts=cu[:1])
+    with pytest.raises(ValueError, match="target_logits"):
+        call(target_logits=z[:4])
+    with pytest.raises(TypeError, match="target_logits"):
+        call(target_logits=z.double())
+    with pytest.raises(ValueError, match="column"):
+        call(target_logits=z[:, :0], draft_probs=None)
+    with pytest.raises(ValueError, match="uniforms"):
+        call(uniforms=u[:2])
+    with pytest.raises(ValueError, match="final_uniforms"):
+        call(final_uniforms=r.double())
+    with pytest.raises(ValueError, match="draft_probs"):
+        call(draft_probs=q[:, :19])
+    with pytest.raises(ValueError, match="temperature"):
+        call(temperature=torch.ones(3))
