@@ -279,6 +279,9 @@ namespace frx {
 // kI8 (with kNH = 1, K-major operands): signed 8-bit operands, kind::i8, int32 accumulators. A
 // 128-byte sub-tile row then holds 128 K elements instead of 64 and one MMA covers K = 32 instead
 // of 16: the same bytes per stage, twice the products.
+// kI8 also has two groups of four epilogue warps, one per TMEM accumulator: a tile's mainloop takes
+// half the time of a 16-bit one, and its epilogue, with the scales to apply, does not; each group has
+// the time of two tiles for one.
 // Either way a stage is 8 MMAs per tcgen05.commit: every commit costs the tensor pipe a drain
 // bubble of roughly one MMA, which at 4 MMAs per commit held the pipe to ~79% busy and at 8 lets
 // it run at ~99%.
@@ -302,8 +305,10 @@ struct PairCfg {
   static constexpr int kTileN = 256 * kNH;
 };
 
+constexpr int kGemmThreadsI8 = kGemmThreads + 128;
+
 template <bool kAMN, bool kBMN, int kNH, class Epi, bool kI8 = false>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8 : kGemmThreads, 1)
     gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                              TileSched sched, int num_k_blocks, const __grid_constant__ typename Epi::Params ep,
                              int* status) {
@@ -359,6 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   tc_fence_before();
   cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated in both
   tc_fence_after();
+  if (kI8) grid_dep_wait();  // the launch may overlap the end of its predecessor, which wrote an operand
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
@@ -498,8 +504,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
   } else {
     // ------------------------------------------------------------------ epilogue warps (both CTAs)
     const int q = warp & 3;
-    int local = 0;
-    for (int t = pair_id; t < sched.num_tiles; t += num_pairs, ++local) {
+    constexpr int kGroups = kI8 ? 2 : 1;
+    const int group = kI8 ? (warp - 2) >> 2 : 0;
+    int local = group;
+    for (int t = pair_id + group * num_pairs; t < sched.num_tiles; t += kGroups * num_pairs, local += kGroups) {
       const int buf = local % Cfg::kNumAcc;
       const uint32_t acc_phase = static_cast<uint32_t>((local / Cfg::kNumAcc) & 1);
       int ok = 1;
@@ -523,10 +531,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         const bool last = h == kNH - 1;
         if (n_blk < sched.n256) {
           if (last) {
-            Epi::run(ep, s_epi + q * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
+            Epi::run(ep, s_epi + (group * 4 + q) * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
                      pm * 2 + static_cast<int>(rank), n_blk, q, lane, release);
           } else {
-            Epi::run(ep, s_epi + q * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
+            Epi::run(ep, s_epi + (group * 4 + q) * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
                      pm * 2 + static_cast<int>(rank), n_blk, q, lane, [] {});
           }
         } else if (last) {

@@ -121,9 +121,28 @@ bool use_pair_kernel();
 // Positive integer from the environment variable `name`, else `fallback` (tuning knobs only).
 int env_int(const char* name, int fallback);
 
+// Launches `kernel`; with `overlap` as a programmatic dependent launch: it may start before its
+// predecessor in the stream (a launch of this library that the kernel waits for with grid_dep_wait) ends.
+template <class... KArgs, class... Args>
+int launch_kernel(void (*kernel)(KArgs...), unsigned grid, unsigned block, int smem, cudaStream_t stream, bool overlap,
+                  Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  FRX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+  return FRX_OK;
+}
+
 // Co-resident 2-CTA clusters of `kernel` on the current device (cached per device).
 template <class Kernel>
-int max_pair_clusters(Kernel kernel, std::atomic<int>* cache, int smem_bytes, int* out) {
+int max_pair_clusters(Kernel kernel, std::atomic<int>* cache, int smem_bytes, int* out, int threads = kGemmThreads) {
   int dev = 0;
   FRX_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 64) {
@@ -135,7 +154,7 @@ int max_pair_clusters(Kernel kernel, std::atomic<int>* cache, int smem_bytes, in
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
-  cfg.blockDim = dim3(kGemmThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem_bytes);
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -153,10 +172,11 @@ int max_pair_clusters(Kernel kernel, std::atomic<int>* cache, int smem_bytes, in
 }
 
 // Launches the pair kernel on signed 8-bit operands: D[m, n] = sum_k a[m, k] b[n, k] in int32, both
-// row-major [extent, K] with 16-byte aligned bases and row strides that are multiples of 16.
+// row-major [extent, K] with 16-byte aligned bases and row strides that are multiples of 16. overlap:
+// the launch directly follows the library's own launch that wrote an operand.
 template <class Epi>
 int launch_gemm_i8(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int64_t M, int64_t N, int64_t K,
-                   int group_m, const typename Epi::Params& ep, int* status, cudaStream_t stream) {
+                   int group_m, const typename Epi::Params& ep, int* status, cudaStream_t stream, bool overlap) {
   using Cfg = PairCfg<1>;
   CUtensorMap tm_a, tm_b;
   int rc = encode_8bit_2d(&tm_a, a, M, K, ld_a, kBM, 128);
@@ -183,13 +203,11 @@ int launch_gemm_i8(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int
   rc = ensure_smem_attr(kernel, attr_done, smem);
   if (rc) return rc;
   int clusters = 0;
-  rc = max_pair_clusters(kernel, clusters_cache, smem, &clusters);
+  rc = max_pair_clusters(kernel, clusters_cache, smem, &clusters, kGemmThreadsI8);
   if (rc) return rc;
   const long long pairs = tiles < clusters ? tiles : clusters;
-  kernel<<<static_cast<unsigned>(2 * pairs), kGemmThreads, smem, stream>>>(tm_a, tm_b, sched, num_k_blocks, ep,
-                                                                           status);
-  FRX_CUDA_CHECK(cudaGetLastError());
-  return FRX_OK;
+  return launch_kernel(kernel, static_cast<unsigned>(2 * pairs), kGemmThreadsI8, smem, stream, overlap, tm_a, tm_b,
+                       sched, num_k_blocks, ep, status);
 }
 
 // Launches the GEMM core. kWide selects 256 x 512 pair tiles (backward GEMMs, long K) instead of

@@ -28,9 +28,11 @@ def _vector(t: Tensor, name: str, n: int, dtype: torch.dtype) -> Tensor:
 def _ids(t: Tensor, name: str) -> Tensor:
     if t.dim() != 1:
         raise ValueError(f"{name} must be 1-D, got shape {tuple(t.shape)}")
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-    return t.to(torch.int64).contiguous()
+    if t.dtype != torch.int64:
+        if t.dtype != torch.int32:
+            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+        t = t.to(torch.int64)
+    return t.contiguous()
 
 
 def _rows(t: Tensor, name: str, n: int, vocab: Optional[int]) -> Tensor:

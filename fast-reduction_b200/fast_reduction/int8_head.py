@@ -49,6 +49,13 @@ def _aligned_codes(codes: Tensor) -> Tensor:
     return out
 
 
+def _rows_2d(x: Tensor) -> Tensor:
+    """x as a matrix of its rows, with unit column stride and rows that do not overlap."""
+    if x.dim() != 2:
+        x = x.reshape(x.shape[:-1].numel(), x.shape[-1])
+    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
 def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
     """8-bit codes of the rows of ``x`` [..., K] (bf16, fp16 or fp32): (codes int8 [..., K], scale fp32 [...])
     with x ~ codes * scale[..., None]. scale = max |row| / 127; each code is the integer nearest to x / scale,
@@ -63,23 +70,16 @@ def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
         raise ValueError("quantize_int8 needs at least one dimension")
     _no_grad_inputs(x)
     ops._require_cuda(x)
-    codes, scale = _quantize_2d(x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(),
-                                                                                         x.shape[-1]))
+    rows = _rows_2d(x) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
+    codes = _codes_like(rows.shape[0], rows.shape[1], x.device)
+    scale = torch.empty(rows.shape[0], device=x.device, dtype=torch.float32)
+    ops.quantize_i8(rows, codes, scale)
     return codes if x.dim() == 2 else codes.reshape(x.shape), scale.view(x.shape[:-1])
-
-
-def _quantize_2d(x: Tensor) -> Tuple[Tensor, Tensor]:
-    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
-        x = x.contiguous()
-    codes = _codes_like(x.shape[0], x.shape[1], x.device)
-    scale = torch.empty(x.shape[0], device=x.device, dtype=torch.float32)
-    ops.quantize_i8(x, codes, scale)
-    return codes, scale
 
 
 def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
              hidden_scale: Optional[Tensor]):
-    """Checked operands: (batch shape, hidden codes [M, K], hidden scale [M], weight codes, weight scale, bias)."""
+    """Checked operands: (hidden [M, H], hidden scale [M] or None, weight codes, weight scale, bias)."""
     if weight_codes.dim() != 2 or weight_codes.dtype != torch.int8:
         raise TypeError(f"weight_codes must be int8 [V, H], got {weight_codes.dtype} {tuple(weight_codes.shape)}")
     V, H = weight_codes.shape
@@ -95,25 +95,23 @@ def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: O
         if bias.dtype not in _FLOATS or bias.shape != (V,):
             raise ValueError(f"bias must be bfloat16, float16 or float32 [{V}], got {bias.dtype} {tuple(bias.shape)}")
         bias = bias.contiguous()
-    batch_shape = hidden.shape[:-1]
     if hidden.dtype == torch.int8:
         if hidden_scale is None:
             raise ValueError("int8 hidden states need hidden_scale (one float32 per token)")
-        if hidden_scale.dtype != torch.float32 or hidden_scale.shape != batch_shape:
-            raise ValueError(f"hidden_scale must be float32 {tuple(batch_shape)}, got {hidden_scale.dtype} "
+        if hidden_scale.dtype != torch.float32 or hidden_scale.shape != hidden.shape[:-1]:
+            raise ValueError(f"hidden_scale must be float32 {tuple(hidden.shape[:-1])}, got {hidden_scale.dtype} "
                              f"{tuple(hidden_scale.shape)}")
+        hidden_scale = hidden_scale.reshape(-1).contiguous()
     elif hidden.dtype not in _FLOATS:
         raise TypeError(f"hidden must be bfloat16, float16, float32 or int8, got {hidden.dtype}")
     elif hidden_scale is not None:
         raise ValueError("hidden_scale goes with int8 hidden states; floating-point ones are quantised here")
     _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
     ops._require_cuda(hidden, weight_codes, weight_scale, bias, hidden_scale)
-    x = hidden.reshape(-1, H)
+    x = _rows_2d(hidden)
     if hidden.dtype == torch.int8:
-        x, x_scale = _aligned_codes(x), hidden_scale.reshape(-1).contiguous()
-    else:
-        x, x_scale = _quantize_2d(x)
-    return batch_shape, x, x_scale, _aligned_codes(weight_codes), weight_scale.contiguous(), bias
+        x = _aligned_codes(x)
+    return x, hidden_scale, _aligned_codes(weight_codes), weight_scale.contiguous(), bias
 
 
 def int8_linear(
@@ -139,16 +137,18 @@ def int8_linear(
         out_dtype = out.dtype if out is not None else (torch.bfloat16 if hidden.dtype == torch.int8 else hidden.dtype)
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-    V = weight_codes.shape[0]
-    rows = hidden.shape[:-1].numel()
-    if out is not None and (out.dtype != out_dtype or out.shape != (rows, V) or (V > 1 and out.stride(1) != 1)
-                            or (rows > 1 and out.stride(0) < V)):
-        raise ValueError(f"out must be {out_dtype} [{rows}, {V}] with unit column stride and rows that do not overlap, "
-                         f"got {out.dtype} {tuple(out.shape)} stride {out.stride()}")
-    batch_shape, x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
+    if out is not None:
+        rows, V = hidden.shape[:-1].numel(), weight_codes.shape[0]
+        if out.dtype != out_dtype or out.shape != (rows, V) or (V > 1 and out.stride(1) != 1) \
+                or (rows > 1 and out.stride(0) < V):
+            raise ValueError(f"out must be {out_dtype} [{rows}, {V}] with unit column stride and rows that do not "
+                             f"overlap, got {out.dtype} {tuple(out.shape)} stride {out.stride()}")
+    x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
+    rows, V = x.shape[0], w.shape[0]
     y = torch.empty(rows, V, device=x.device, dtype=out_dtype) if out is None else out
-    ops.gemm_i8(x, x_scale, w, w_scale, y, bias=bias)
-    return y.view(*batch_shape, V) if out is None else out
+    workspace = torch.empty(ops.i8_workspace_bytes(x), device=x.device, dtype=torch.uint8)
+    ops.gemm_i8(x, x_scale, w, w_scale, y, workspace, bias=bias)
+    return y if out is not None or hidden.dim() == 2 else y.view(*hidden.shape[:-1], V)
 
 
 def int8_ce_entropy(
@@ -166,26 +166,25 @@ def int8_ce_entropy(
     int8_linear would give in fp32, which never reach HBM. Operands as in int8_linear; target, chunk_size and
     ignore_index as in gemm_fused_ce_entropy (ignored rows: ce = log_probs = 0, entropy kept; a target
     outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET)."""
-    batch_shape, x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
-    target = target.reshape(-1)
+    x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
     B = x.shape[0]
     if target.numel() != B:
         raise ValueError(f"target has {target.numel()} elements, expected {B}")
-    if target.dtype.is_floating_point or target.dtype.is_complex or target.dtype == torch.bool:
-        raise TypeError(f"target must be an integer tensor, got {target.dtype}")
-    target = target.to(torch.int64).contiguous()
-    ops._require_cuda(x, target)
-    ce, ent, logp = (torch.empty(B, device=x.device, dtype=torch.float32) for _ in range(3))
+    if target.dtype != torch.int64:
+        if target.dtype.is_floating_point or target.dtype.is_complex or target.dtype == torch.bool:
+            raise TypeError(f"target must be an integer tensor, got {target.dtype}")
+        target = target.to(torch.int64)
+    target = target.contiguous()
     chunk = gk._chunk_rows(chunk_size, B)
+    dev = x.device
+    ce, ent, logp = torch.empty(3, B, device=dev, dtype=torch.float32).unbind(0)
     if B:
-        V = w.shape[0]
-        T = ops.n_vocab_tiles(V)
-        chunk = gk._launch_rows(chunk, B, T)
-        partials = torch.empty(T, chunk, 4, device=x.device, dtype=torch.float32)
-        for a in range(0, B, chunk):
-            b = min(a + chunk, B)
-            with ops.phase("frx.int8.chunk"):
-                ops.fwd_partials_i8(x[a:b], x_scale[a:b], w, w_scale, target[a:b], partials, chunk, bias=bias)
-            ops.finalize(partials, T, b - a, chunk, target=target[a:b], vocab_size=V, ignore_index=ignore_index,
-                         ce=ce[a:b], entropy=ent[a:b], log_probs=logp[a:b])
-    return ce.view(batch_shape), ent.view(batch_shape), logp.view(batch_shape)
+        tiles = ops.n_vocab_tiles(w.shape[0])
+        chunk = gk._launch_rows(chunk, B, tiles)
+        workspace = torch.empty(ops.i8_workspace_bytes(x) + 16 * tiles * chunk, device=dev, dtype=torch.uint8)
+        ops.i8_ce_entropy(x, x_scale, w, w_scale, target, ce, ent, logp, workspace, launch_rows=chunk,
+                          ignore_index=ignore_index, bias=bias)
+    if hidden.dim() == 2:
+        return ce, ent, logp
+    shape = hidden.shape[:-1]
+    return ce.view(shape), ent.view(shape), logp.view(shape)

@@ -473,6 +473,17 @@ def scale_inplace(x: torch.Tensor, scale: torch.Tensor) -> None:
     nat.check(rc, "frx_scale_inplace")
 
 
+# Device work of the functions below runs on the tensors' device whatever the current one is.
+def _launch_on(name: str, dev: torch.device, call) -> int:
+    if dev.index == torch.cuda.current_device():
+        return _launch(name, dev, call)
+    with torch.cuda.device(dev):
+        return _launch(name, dev, call)
+
+
+_I8_X_DTYPES = {**_OUT_DTYPES, torch.int8: nat.FRX_DTYPE_I8}
+
+
 def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
     """codes (int8), scale (fp32 per row) <- symmetric 8-bit codes of the rows of x (frx_quantize_i8)."""
     dev = _require_cuda(x, codes, scale)
@@ -481,63 +492,72 @@ def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> No
     if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
         raise ValueError("codes must have x's shape and scale one value per row")
     lib = nat.load()
-    with torch.cuda.device(dev):
-        rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
-            x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
-            scale.data_ptr(), nat.stream_of(dev)))
+    rc = _launch_on("quantize_i8", dev, lambda: lib.frx_quantize_i8(
+        x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
+        scale.data_ptr(), nat.stream_of(dev)))
     nat.check(rc, "frx_quantize_i8")
 
 
+def i8_workspace_bytes(x: torch.Tensor) -> int:
+    """Workspace of a product whose tokens are ``x`` [rows, k]: their codes and scales, unless they are codes."""
+    return 0 if x.dtype == torch.int8 else round_up(x.shape[0] * (round_up(x.shape[1], 16) + 4), 16)
+
+
 def _i8_operands(x, x_scale, weight, weight_scale, bias):
-    if x.dtype != torch.int8 or weight.dtype != torch.int8:
-        raise TypeError(f"codes must be int8, got {x.dtype} and {weight.dtype}")
+    """Checked operands of an 8-bit product: (device, the leading C arguments up to bias_dtype)."""
+    dev = _require_cuda(x, x_scale, weight, weight_scale, bias)
+    if x.dtype not in _I8_X_DTYPES or weight.dtype != torch.int8:
+        raise TypeError(f"x must be int8, bfloat16, float16 or float32 and weight int8, got {x.dtype} and {weight.dtype}")
     ldx, ldw = _row_major(x, "x"), _row_major(weight, "weight")
-    if x.shape[1] != weight.shape[1]:
+    rows, k = x.shape
+    cols = weight.shape[0]
+    if weight.shape[1] != k:
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
-    for name, t, n in (("x_scale", x_scale, x.shape[0]), ("weight_scale", weight_scale, weight.shape[0])):
-        if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous float32 [{n}]")
-    if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (weight.shape[0],)
-                             or not bias.is_contiguous()):
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (cols,) or not weight_scale.is_contiguous():
+        raise ValueError(f"weight_scale must be contiguous float32 [{cols}]")
+    if (x_scale is None) != (x.dtype != torch.int8) or (x_scale is not None and (
+            x_scale.dtype != torch.float32 or x_scale.shape != (rows,) or not x_scale.is_contiguous())):
+        raise ValueError(f"x_scale must be contiguous float32 [{rows}] for int8 x, and None otherwise")
+    if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (cols,) or not bias.is_contiguous()):
         raise ValueError("bias must be a contiguous bfloat16, float16 or float32 vector with one value per weight row")
-    return ldx, ldw, 0 if bias is None else _OUT_DTYPES[bias.dtype]
+    return dev, (x.data_ptr(), _I8_X_DTYPES[x.dtype], max(ldx, k), nat.ptr(x_scale), weight.data_ptr(), max(ldw, k),
+                 weight_scale.data_ptr(), nat.ptr(bias), 0 if bias is None else _OUT_DTYPES[bias.dtype])
 
 
-def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
-            out: torch.Tensor, *, bias: torch.Tensor | None = None) -> None:
-    """out[r, j] <- (x[r] . weight[j]) * x_scale[r] * weight_scale[j] (+ bias[j]) for int8 codes (frx_gemm_i8)."""
-    dev = _require_cuda(x, x_scale, weight, weight_scale, bias, out)
-    ldx, ldw, bdt = _i8_operands(x, x_scale, weight, weight_scale, bias)
-    if out.dtype not in _OUT_DTYPES or out.shape != (x.shape[0], weight.shape[0]):
-        raise ValueError(f"out must be bfloat16, float16 or float32 [{x.shape[0]}, {weight.shape[0]}]")
+def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
+            out: torch.Tensor, workspace: torch.Tensor | None, *, bias: torch.Tensor | None = None) -> None:
+    """out[r, j] <- (xc[r] . weight[j]) * x_scale[r] * weight_scale[j] (+ bias[j]): xc = x for int8 x, else its codes,
+    which go into the uint8 ``workspace`` (frx_gemm_i8)."""
+    dev, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
+    rows, cols = x.shape[0], weight.shape[0]
+    if out.dtype not in _OUT_DTYPES or out.shape != (rows, cols) or out.device != dev:
+        raise ValueError(f"out must be bfloat16, float16 or float32 [{rows}, {cols}] on {dev}")
     lib = nat.load()
-    with torch.cuda.device(dev):
-        rc = _launch("gemm_i8", dev, lambda: lib.frx_gemm_i8(
-            x.data_ptr(), ldx, x_scale.data_ptr(), weight.data_ptr(), ldw, weight_scale.data_ptr(), nat.ptr(bias), bdt,
-            x.shape[0], weight.shape[0], x.shape[1], out.data_ptr(), max(out.stride(0), out.shape[1]),
-            _OUT_DTYPES[out.dtype], nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    rc = _launch_on("gemm_i8", dev, lambda: lib.frx_gemm_i8(
+        *operands, rows, cols, x.shape[1], nat.ptr(workspace), 0 if workspace is None else workspace.numel(),
+        out.data_ptr(), max(out.stride(0), cols), _OUT_DTYPES[out.dtype], nat.status_word(dev).data_ptr(),
+        nat.stream_of(dev)))
     nat.check(rc, "frx_gemm_i8")
 
 
-def fwd_partials_i8(hidden: torch.Tensor, hidden_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
-                    target: torch.Tensor | None, partials: torch.Tensor, tile_stride: int, vocab_offset: int = 0, *,
-                    bias: torch.Tensor | None = None) -> None:
-    """fwd_partials of the logits gemm_i8 would give (frx_fwd_partials_i8)."""
-    dev = _require_cuda(hidden, hidden_scale, weight, weight_scale, target, partials, bias)
-    ldh, ldw, bdt = _i8_operands(hidden, hidden_scale, weight, weight_scale, bias)
-    rows, vshard = hidden.shape[0], weight.shape[0]
-    if target is not None and (target.dtype != torch.int64 or not target.is_contiguous() or target.numel() < rows):
+def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
+                  target: torch.Tensor, ce: torch.Tensor, entropy: torch.Tensor, log_probs: torch.Tensor,
+                  workspace: torch.Tensor, *, launch_rows: int, ignore_index: int,
+                  bias: torch.Tensor | None = None) -> None:
+    """ce, entropy, log_probs <- those of gemm_i8's fp32 logits, launch_rows rows at a time (frx_i8_ce_entropy)."""
+    dev, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
+    rows = x.shape[0]
+    if target.dtype != torch.int64 or not target.is_contiguous() or target.numel() != rows or target.device != dev:
         raise ValueError("target must be a contiguous int64 tensor with one id per row")
-    if partials.dtype != torch.float32 or not partials.is_contiguous() or tile_stride < rows or \
-            partials.numel() < 4 * ((n_vocab_tiles(vshard) - 1) * tile_stride + rows):
-        raise ValueError("partials must be contiguous float32 covering every tile of the launch")
+    for name, t in (("ce", ce), ("entropy", entropy), ("log_probs", log_probs)):
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != rows:
+            raise ValueError(f"{name} must be contiguous float32 with one value per row")
     lib = nat.load()
-    with torch.cuda.device(dev):
-        rc = _launch("fwd_partials_i8", dev, lambda: lib.frx_fwd_partials_i8(
-            hidden.data_ptr(), ldh, hidden_scale.data_ptr(), weight.data_ptr(), ldw, weight_scale.data_ptr(),
-            nat.ptr(bias), bdt, nat.ptr(target), rows, vshard, hidden.shape[1], vocab_offset, partials.data_ptr(),
-            tile_stride, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
-    nat.check(rc, "frx_fwd_partials_i8")
+    rc = _launch_on("i8_ce_entropy", dev, lambda: lib.frx_i8_ce_entropy(
+        *operands, target.data_ptr(), rows, weight.shape[0], x.shape[1], ignore_index, launch_rows,
+        workspace.data_ptr(), workspace.numel(), ce.data_ptr(), entropy.data_ptr(), None, log_probs.data_ptr(),
+        nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    nat.check(rc, "frx_i8_ce_entropy")
 
 
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor, uniforms: torch.Tensor,
@@ -566,11 +586,10 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
     if workspace.dtype != torch.float32 or not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous float32")
     lib = nat.load()
-    with torch.cuda.device(dev):
-        rc = _launch("verify_drafts", dev, lambda: lib.frx_verify_drafts(
-            logits.data_ptr(), _LOGITS_DTYPES[logits.dtype], ldl, drafts.data_ptr(), cu_drafts.data_ptr(),
-            uniforms.data_ptr(), final_uniforms.data_ptr(), nat.ptr(draft_probs),
-            0 if draft_probs is None else _LOGITS_DTYPES[draft_probs.dtype], ldq, nat.ptr(temperature),
-            temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
-            tokens.data_ptr(), log_probs.data_ptr(), nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    rc = _launch_on("verify_drafts", dev, lambda: lib.frx_verify_drafts(
+        logits.data_ptr(), _LOGITS_DTYPES[logits.dtype], ldl, drafts.data_ptr(), cu_drafts.data_ptr(),
+        uniforms.data_ptr(), final_uniforms.data_ptr(), nat.ptr(draft_probs),
+        0 if draft_probs is None else _LOGITS_DTYPES[draft_probs.dtype], ldq, nat.ptr(temperature),
+        temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
+        tokens.data_ptr(), log_probs.data_ptr(), nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
     nat.check(rc, "frx_verify_drafts")

@@ -48,6 +48,7 @@ extern "C" {
 #define FRX_DTYPE_BF16 0
 #define FRX_DTYPE_F32 1
 #define FRX_DTYPE_F16 2
+#define FRX_DTYPE_I8 3 /* signed 8-bit codes (the operands of frx_gemm_i8 and frx_i8_ce_entropy) */
 
 /* Or-ed into the out_dtype of frx_gemm_dhidden / frx_gemm_dweight with FRX_DTYPE_F32: the product is
  * added to the fp32 values the output already holds (several launches accumulate one result). */
@@ -309,25 +310,36 @@ FRX_API int frx_quantize_i8(const void* x, int dtype, int64_t ld_x, int64_t rows
                             int64_t ld_codes, float* scale, void* stream);
 
 /*
- * out[r, j] = (sum_c x[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]) for signed 8-bit codes
- * x [rows, k] and weight [cols, k] (row strides ld_x, ld_weight: multiples of 16, bases 16-byte aligned):
- * exact int32 sums (k <= 131072, codes within +-127), scaled in fp32 and rounded once to out_dtype (BF16,
- * F16 or F32; any ld_out >= cols and any alignment of the element type). bias (bias_dtype BF16, F16 or
- * F32) may be NULL. No counterpart in the reference.
- */
-FRX_API int frx_gemm_i8(const void* x, int64_t ld_x, const float* x_scale, const void* weight, int64_t ld_weight,
-                        const float* weight_scale, const void* bias, int bias_dtype, int64_t rows, int64_t cols,
-                        int64_t k, void* out, int64_t ld_out, int out_dtype, int* status, void* stream);
-
-/*
- * frx_fwd_partials on 8-bit codes: the logits of frx_gemm_i8, reduced to the same (m, s, u, zt) partials by
- * the epilogue; frx_finalize merges them. Operands as in frx_gemm_i8, the rest as in frx_fwd_partials.
+ * out[r, j] = (sum_c xc[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]), with xc and weight [cols, k]
+ * signed 8-bit codes within +-127: exact int32 sums (k <= 131072), scaled in fp32 and rounded once to
+ * out_dtype (BF16, F16 or F32; any ld_out >= cols and any alignment of the element type).
+ *   x_dtype    FRX_DTYPE_I8: x holds the codes, x_scale [rows] their scales. FRX_DTYPE_BF16, _F16 or _F32: x is
+ *              quantised as by frx_quantize_i8 into the workspace first (x_scale is not read)
+ *   codes      16-byte aligned bases, row strides that are multiples of 16
+ *   bias       optional [cols], bias_dtype BF16, F16 or F32
+ *   workspace  for floating-point x: round_up(rows * (round_up(k, 16) + 4), 16) bytes, 16-byte aligned; calls
+ *              that overlap need one each. Not read for FRX_DTYPE_I8
  * No counterpart in the reference.
  */
-FRX_API int frx_fwd_partials_i8(const void* hidden, int64_t ld_hidden, const float* hidden_scale, const void* weight,
-                                int64_t ld_weight, const float* weight_scale, const void* bias, int bias_dtype,
-                                const int64_t* target, int64_t rows, int64_t vocab_shard, int64_t hidden_dim,
-                                int64_t vocab_offset, float* partials, int64_t tile_stride, int* status, void* stream);
+FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x_scale, const void* weight,
+                        int64_t ld_weight, const float* weight_scale, const void* bias, int bias_dtype, int64_t rows,
+                        int64_t cols, int64_t k, void* workspace, int64_t workspace_bytes, void* out, int64_t ld_out,
+                        int out_dtype, int* status, void* stream);
+
+/*
+ * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
+ * HBM: the product's epilogue reduces them to the partials of frx_fwd_partials and frx_finalize merges those,
+ * launch_rows rows at a time. Operands as in frx_gemm_i8, target rules as in frx_finalize.
+ *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
+ *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes
+ * No counterpart in the reference.
+ */
+FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_hidden, const float* hidden_scale,
+                              const void* weight, int64_t ld_weight, const float* weight_scale, const void* bias,
+                              int bias_dtype, const int64_t* target, int64_t rows, int64_t vocab_size,
+                              int64_t hidden_dim, int64_t ignore_index, int64_t launch_rows, void* workspace,
+                              int64_t workspace_bytes, float* ce, float* entropy, float* lse, float* log_probs,
+                              int* status, void* stream);
 
 /*
  * Verifies drafted tokens against the target model's logits (speculative sampling) from given random

@@ -32,15 +32,15 @@ ARGTYPES = {
     "frx_gemm_dhidden_multicast": [P, I64, P, I64, I32, P, I64, I64, I64, I64, P, P],
     "frx_test_stalled_fwd": [P, I64, P, I64, P, I64, I64, I64, P, I64, I32, I64, P, P],
     "frx_quantize_i8": [P, I32, I64, I64, I64, P, I64, P, P],
-    "frx_gemm_i8": [P, I64, P, P, I64, P, P, I32, I64, I64, I64, P, I64, I32, P, P],
-    "frx_fwd_partials_i8": [P, I64, P, P, I64, P, P, I32, P, I64, I64, I64, I64, P, I64, P, P],
+    "frx_gemm_i8": [P, I32, I64, P, P, I64, P, P, I32, I64, I64, I64, P, I64, P, I64, I32, P, P],
+    "frx_i8_ce_entropy": [P, I32, I64, P, P, I64, P, P, I32, P, I64, I64, I64, I64, I64, P, I64, P, P, P, P, P, P],
     "frx_verify_drafts": [P, I32, I64, P, P, P, P, P, I32, I64, P, F32, I64, I64, I64, P, I64, P, P, P, P, P],
     "frx_check_range": [P, I64],
     "frx_clock_probe": [P, I32, P],
     "frx_abi_version": [],
 }
 
-FRX_DTYPE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+FRX_DTYPE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2, torch.int8: 3}
 NO_IGNORE = -(2**63)  # an ignore_index no target equals (the reference kernels have no ignore rule)
 
 _lib = None
@@ -186,22 +186,27 @@ def quantize_i8(X, codes, scale):
                                 codes.stride(0), scale.data_ptr(), _stream(X)))
 
 
-def gemm_i8(Xq, x_scale, Wq, w_scale, out, *, bias=None):
-    """Logits of 8-bit codes (row strides multiples of 16) with scales per row of each operand."""
-    M, K = Xq.shape
+def gemm_i8(X, x_scale, Wq, w_scale, out, workspace, *, bias=None):
+    """Logits against 8-bit codes Wq (row stride a multiple of 16) with a scale per row. X: int8 codes with x_scale, or
+    float rows, quantised into the uint8 workspace (include/frx.h gives its size; None for codes)."""
+    M, K = X.shape
     V = Wq.shape[0]
-    _check(_lib.frx_gemm_i8(Xq.data_ptr(), Xq.stride(0), x_scale.data_ptr(), Wq.data_ptr(), Wq.stride(0),
+    _check(_lib.frx_gemm_i8(X.data_ptr(), FRX_DTYPE[X.dtype], X.stride(0), _ptr(x_scale), Wq.data_ptr(), Wq.stride(0),
                             w_scale.data_ptr(), _ptr(bias), 0 if bias is None else FRX_DTYPE[bias.dtype], M, V, K,
-                            out.data_ptr(), out.stride(0), FRX_DTYPE[out.dtype], None, _stream(Xq)))
+                            _ptr(workspace), 0 if workspace is None else workspace.numel(), out.data_ptr(),
+                            out.stride(0), FRX_DTYPE[out.dtype], None, _stream(X)))
 
 
-def fwd_partials_i8(Aq, a_scale, Wq, w_scale, target, partials, *, bias=None, vocab_offset=0):
-    """fwd_partials on 8-bit codes; partials: fp32 [ceil(V / 256), M, 4]."""
-    M, K = Aq.shape
+def i8_ce_entropy(X, x_scale, Wq, w_scale, target, ce, entropy, log_probs, workspace, *, bias=None, launch_rows=4096,
+                  ignore_index=-100):
+    """CE, entropy and log-probabilities of gemm_i8's logits, which stay on the chip."""
+    M, K = X.shape
     V = Wq.shape[0]
-    _check(_lib.frx_fwd_partials_i8(Aq.data_ptr(), Aq.stride(0), a_scale.data_ptr(), Wq.data_ptr(), Wq.stride(0),
-                                    w_scale.data_ptr(), _ptr(bias), 0 if bias is None else FRX_DTYPE[bias.dtype],
-                                    _ptr(target), M, V, K, vocab_offset, partials.data_ptr(), M, None, _stream(Aq)))
+    _check(_lib.frx_i8_ce_entropy(X.data_ptr(), FRX_DTYPE[X.dtype], X.stride(0), _ptr(x_scale), Wq.data_ptr(),
+                                  Wq.stride(0), w_scale.data_ptr(), _ptr(bias),
+                                  0 if bias is None else FRX_DTYPE[bias.dtype], target.data_ptr(), M, V, K,
+                                  ignore_index, launch_rows, workspace.data_ptr(), workspace.numel(), ce.data_ptr(),
+                                  entropy.data_ptr(), None, log_probs.data_ptr(), None, _stream(X)))
 
 
 def verify_drafts(L, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature, workspace, accepted, tokens,

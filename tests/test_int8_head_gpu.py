@@ -289,3 +289,28 @@ def test_other_stream_and_two_streams_at_once():
     torch.cuda.synchronize()
     for y, sc in got:
         assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(sc, score))
+
+
+@pytest.mark.parametrize("rows", [5, 200])
+def test_zero_negative_and_uneven_scales(rows):
+    """Zero rows and weights, and the caller's own scales: negative, zero, and far apart."""
+    from fast_reduction import int8_ce_entropy, int8_linear
+
+    g = _gen(14)
+    k, v = 80, 1100
+    x = torch.randint(-127, 128, (rows, k), device=DEV, generator=g, dtype=torch.int8)
+    w = torch.randint(-127, 128, (v, k), device=DEV, generator=g, dtype=torch.int8)
+    x[0] = 0
+    w[:3] = 0
+    xs = torch.logspace(-4, 0, rows, device=DEV) * 1e-3
+    xs[1], xs[2], xs[3] = -xs[1], 0.0, -1e-3
+    ws = (torch.rand(v, device=DEV, generator=g) + 0.5) * 0.1
+    ws[700:] = -ws[700:]
+    t = torch.randint(0, v, (rows,), device=DEV, generator=g)
+    for bias in (None, torch.randn(v, device=DEV, generator=g)):
+        z, mag = ref_logits(x, xs, w, ws, bias)
+        assert_logits(int8_linear(x, w, ws, bias=bias, hidden_scale=xs, out_dtype=torch.float32), z, mag)
+        ce, ent, _ = int8_ce_entropy(x, w, ws, t, bias=bias, hidden_scale=xs)
+        ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, t)
+        assert ((ce.double() - ce_r).abs() <= tol_ce).all()
+        assert ((ent.double() - ent_r).abs() <= tol_ent).all()

@@ -28,24 +28,30 @@ def test_quantize_entry_point():
 def test_product_entry_points(score):
     nat, lib = _lib()
 
-    def call(x=A, ld_x=64, xs=B, w=C, ld_w=64, ws=D, bias=None, bdt=0, rows=4, cols=8, k=64, out=A, ld=8, odt=0):
+    def call(x=A, xdt=nat.FRX_DTYPE_I8, ld_x=64, xs=B, w=C, ld_w=64, ws=D, bias=None, bdt=0, rows=4, cols=8, k=64,
+             out=A, ld=8, odt=0, work=B, nbytes=1 << 20, target=A, step=4):
         if score:
-            return lib.frx_fwd_partials_i8(x, ld_x, xs, w, ld_w, ws, bias, bdt, None, rows, cols, k, 0, out, ld, None,
-                                           None)
-        return lib.frx_gemm_i8(x, ld_x, xs, w, ld_w, ws, bias, bdt, rows, cols, k, out, ld, odt, None, None)
+            return lib.frx_i8_ce_entropy(x, xdt, ld_x, xs, w, ld_w, ws, bias, bdt, target, rows, cols, k, -100, step,
+                                         work, nbytes, A, A, None, A, None, None)
+        return lib.frx_gemm_i8(x, xdt, ld_x, xs, w, ld_w, ws, bias, bdt, rows, cols, k, work, nbytes, out, ld, odt,
+                               None, None)
 
     bad = nat.FRX_ERR_INVALID_ARG
     assert call(rows=-1) == bad and call(cols=0) == bad and call(k=0) == bad and call(rows=1 << 31) == bad
     assert call(k=131073, ld_x=131088, ld_w=131088) == nat.FRX_ERR_UNSUPPORTED
     assert call(x=None) == bad and call(xs=None) == bad and call(w=None) == bad and call(ws=None) == bad
     assert call(x=A + 8) == bad and call(w=C + 1) == bad and call(ld_x=72) == bad and call(ld_w=48) == bad
-    assert call(bias=A, bdt=7) == bad
-    assert call(out=None) == bad
+    assert call(xdt=4) == bad and call(bias=A, bdt=7) == bad and call(bias=A, bdt=nat.FRX_DTYPE_I8) == bad
+    # floating-point tokens need room for their codes (64 bytes a row here) and scales
+    need = 4 * (64 + 4) + (16 * 4 if score else 0)
+    assert call(xdt=0, nbytes=need - 1) == bad and b"workspace" in lib.frx_last_error()
+    assert call(xdt=0, work=None) == bad and call(xdt=0, work=B + 8) == bad and call(xdt=0, ld_x=63) == bad
     assert call(rows=0) == nat.FRX_OK
     if score:
-        assert call(ld=3) == bad and call(out=A + 4) == bad  # tile_stride < rows; unaligned partials
+        assert call(target=None) == bad and call(step=0) == bad
+        assert call(nbytes=16 * 4 - 1) == bad
     else:
-        assert call(ld=7) == bad and call(odt=9) == bad
+        assert call(out=None) == bad and call(ld=7) == bad and call(odt=9) == bad
 
 
 def test_verify_entry_point():
