@@ -279,9 +279,10 @@ namespace frx {
 // kI8 (with kNH = 1, K-major operands): signed 8-bit operands, kind::i8, int32 accumulators. A
 // 128-byte sub-tile row then holds 128 K elements instead of 64 and one MMA covers K = 32 instead
 // of 16: the same bytes per stage, twice the products.
-// kI8 also has two groups of four epilogue warps, one per TMEM accumulator: a tile's mainloop takes
-// half the time of a 16-bit one, and its epilogue, with the scales to apply, does not; each group has
-// the time of two tiles for one.
+// kI8 also has 16 epilogue warps: per TMEM accumulator two groups of four, each on 128 of its columns. A
+// tile's mainloop takes half the time of a 16-bit one while its epilogue has the scales to apply on top;
+// one warp alone issues an instruction every 5 to 6 cycles (dependences), so it is warps that the
+// scheduler lacks (K = 1024, 1024 rows, 32000 columns: 57 us with 8 epilogue warps).
 // Either way a stage is 8 MMAs per tcgen05.commit: every commit costs the tensor pipe a drain
 // bubble of roughly one MMA, which at 4 MMAs per commit held the pipe to ~79% busy and at 8 lets
 // it run at ~99%.
@@ -305,7 +306,17 @@ struct PairCfg {
   static constexpr int kTileN = 256 * kNH;
 };
 
-constexpr int kGemmThreadsI8 = kGemmThreads + 128;
+constexpr int kGemmThreadsI8 = 64 + 16 * 32;
+
+// What an 8-bit epilogue fetches before its tile is ready.
+template <class Epi, bool kI8>
+struct EpiTile {
+  using type = int;
+};
+template <class Epi>
+struct EpiTile<Epi, true> {
+  using type = typename Epi::Tile;
+};
 
 template <bool kAMN, bool kBMN, int kNH, class Epi, bool kI8 = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8 : kGemmThreads, 1)
@@ -314,6 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
                              int* status) {
   using Cfg = PairCfg<kNH>;
   static_assert(!kI8 || (!kAMN && !kBMN && kNH == 1), "8-bit operands are K-major in 256 x 256 tiles");
+  constexpr uint32_t kHint = kI8 ? kSuspendHintShortNs : kSuspendHintNs;
   constexpr int kSubK = kI8 ? 128 : 64;  // K elements of one 128-byte sub-tile row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -325,7 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
   uint64_t* acc_full = empty + Cfg::kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* mma_done = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* join = mma_done + 1;  // kI8: one per pair of epilogue warps that share their rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(join + (kI8 ? 8 : 0));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // uniform over the grid (both CTAs of every pair), so an early return skips every barrier together
   if (!device_check(reinterpret_cast<const uint8_t*>(tmem_slot + 2) - smem_raw <=
@@ -347,9 +360,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);  // one arrival per epilogue warp of both CTAs
+      mbar_init(&acc_empty[b], kI8 ? 16 : 8);  // one arrival per epilogue warp of both CTAs
     }
     mbar_init(mma_done, 1);
+    for (int j = 0; j < (kI8 ? 8 : 0); ++j) mbar_init(&join[j], 1);
     *abort_flag = 0;
     fence_mbarrier_init();
   }
@@ -364,7 +378,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
   tc_fence_before();
   cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated in both
   tc_fence_after();
-  if (kI8) grid_dep_wait();  // the launch may overlap the end of its predecessor, which wrote an operand
+  if (kI8) {
+    grid_dep_launch();  // the successor (the merge of the partials) may start its own prologue
+    grid_dep_wait();    // the launch may overlap the end of its predecessor, which wrote an operand
+  }
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
@@ -381,7 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const int n0 = pn * Cfg::kTileN + static_cast<int>(rank) * 128;
         for (int kb = 0; kb < num_k_blocks; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, status, kStatusTimeoutProducer,
-                                 sched.wait_limit_ns)) {
+                                 sched.wait_limit_ns, kHint)) {
             ok = false;
             break;
           }
@@ -456,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const int buf = local % Cfg::kNumAcc;
         const uint32_t acc_phase = static_cast<uint32_t>((local / Cfg::kNumAcc) & 1);
         if (!mbar_wait_bounded(&acc_empty[buf], acc_phase ^ 1u, abort_flag, status, kStatusTimeoutMma,
-                               sched.wait_limit_ns)) {
+                               sched.wait_limit_ns, kHint)) {
           ok = false;
           break;
         }
@@ -464,7 +481,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * 256);
         for (int kb = 0; kb < num_k_blocks; ++kb) {
           if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma,
-                                 sched.wait_limit_ns)) {
+                                 sched.wait_limit_ns, kHint)) {
             ok = false;
             break;
           }
@@ -504,42 +521,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
   } else {
     // ------------------------------------------------------------------ epilogue warps (both CTAs)
     const int q = warp & 3;
-    constexpr int kGroups = kI8 ? 2 : 1;
-    const int group = kI8 ? (warp - 2) >> 2 : 0;
+    constexpr int kGroups = kI8 ? 2 : 1;  // each takes every second tile, from its own accumulator
+    const int group = kI8 ? ((warp - 2) >> 2) & 1 : 0;
+    const int half = kI8 ? (warp - 2) >> 3 : 0;  // which 128 columns of a tile
+    uint32_t joins = 0;  // parity of this warp pair's next join
+    [[maybe_unused]] typename EpiTile<Epi, kI8>::type tile{}, next{};
+    if constexpr (kI8) {
+      if (pair_id + group * num_pairs < sched.num_tiles) {
+        int pm, pn;
+        sched.get(pair_id + group * num_pairs, pm, pn);
+        tile = Epi::fetch(ep, pm * 2 + static_cast<int>(rank), pn, half, q, lane);
+      }
+    }
     int local = group;
     for (int t = pair_id + group * num_pairs; t < sched.num_tiles; t += kGroups * num_pairs, local += kGroups) {
       const int buf = local % Cfg::kNumAcc;
       const uint32_t acc_phase = static_cast<uint32_t>((local / Cfg::kNumAcc) & 1);
+      int pm, pn;
+      sched.get(t, pm, pn);
+      if constexpr (kI8) {
+        // what the epilogue reads from memory: this tile's into shared memory, the next one's requested
+        Epi::stage(tile, s_epi, group, half, q, lane);
+        if (t + kGroups * num_pairs < sched.num_tiles) {
+          int nm, nn;
+          sched.get(t + kGroups * num_pairs, nm, nn);
+          next = Epi::fetch(ep, nm * 2 + static_cast<int>(rank), nn, half, q, lane);
+        }
+      }
       int ok = 1;
       if (lane == 0)
         ok = mbar_wait_bounded(&acc_full[buf], acc_phase, abort_flag, status, kStatusTimeoutEpilogue,
-                                   sched.wait_limit_ns) ? 1 : 0;
+                                   sched.wait_limit_ns, kHint) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      int pm, pn;
-      sched.get(t, pm, pn);
       const uint32_t tacc = tmem_base + static_cast<uint32_t>(buf * 256) + (static_cast<uint32_t>(q * 32) << 16);
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+        if (lane == 0) {
+          const uint32_t bar = map_to_cta(smem_u32(&acc_empty[buf]), 0);
+          if (kI8)
+            mbar_arrive_cluster_cta(bar);
+          else
+            mbar_arrive_cluster(bar);
+        }
       };
+      if constexpr (kI8) {
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          int done = 1;
+          if (lane == 0)
+            done = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, sched.wait_limit_ns, kHint);
+          return __shfl_sync(0xffffffffu, done, 0) != 0;
+        };
+        if (!Epi::run(ep, tile, s_epi, tacc + static_cast<uint32_t>(half * 128), pm * 2 + static_cast<int>(rank), pn,
+                      group, half, q, lane, &join[group * 4 + q], joins, release, wait))
+          break;
+        tile = next;
+      } else {
 #pragma unroll 1
       for (int h = 0; h < kNH; ++h) {
         const int n_blk = pn * kNH + h;  // 256-column block index
         const bool last = h == kNH - 1;
         if (n_blk < sched.n256) {
           if (last) {
-            Epi::run(ep, s_epi + (group * 4 + q) * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
+            Epi::run(ep, s_epi + q * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
                      pm * 2 + static_cast<int>(rank), n_blk, q, lane, release);
           } else {
-            Epi::run(ep, s_epi + (group * 4 + q) * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
+            Epi::run(ep, s_epi + q * Epi::kSmemPerWarp, tacc + static_cast<uint32_t>(h * 256),
                      pm * 2 + static_cast<int>(rank), n_blk, q, lane, [] {});
           }
         } else if (last) {
           release();
         }
+      }
       }
     }
     Epi::finish(ep, lane);

@@ -36,6 +36,11 @@ void set_error(const char* fmt, ...);
     }                                                                                           \
   } while (0)
 
+// The merge of frx_finalize as a dependent of the launch that wrote the partials (frx_finalize.cu).
+int launch_finalize_dep(const float* partials, int64_t n_tiles, int64_t rows, int64_t tile_stride,
+                        const int64_t* target, int64_t vocab_size, int64_t ignore_index, float* ce, float* entropy,
+                        float* lse, float* log_probs, int* status, cudaStream_t stream);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Number of SMs of the current device (cached per device ordinal).

@@ -20,11 +20,22 @@ namespace frx {
 constexpr int64_t kI8MaxK = 131072;
 
 // ------------------------------------------------------------------------------------ quantisation
-// Eight consecutive values of a row as they lie in memory, and as floats.
+// Eight consecutive values of a row as they lie in memory. max_bits folds the bits of |x| into a running
+// maximum: as integers they order as the values do, with infinity and NaN above every finite one.
 template <typename T>
-struct Raw8 {  // 16-bit types
+struct Raw8 {  // 16-bit types; two maxima per word
   uint4 q;
   __device__ void load(const T* p) { q = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ uint32_t max_bits(uint32_t m) const {
+    const uint32_t a = __vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu);
+    const uint32_t b = __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu);
+    return __vmaxu2(m, __vmaxu2(a, b));
+  }
+  __device__ static uint32_t one_bits(const T* p) { return __ldg(reinterpret_cast<const uint16_t*>(p)) & 0x7fffu; }
+  // the largest |x| of a folded word
+  __device__ static float amax(uint32_t m) {
+    return unpack2(max(m & 0xffffu, m >> 16), std::is_same<T, __half>::value).x;
+  }
   __device__ void floats(float (&v)[8]) const {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -37,26 +48,30 @@ struct Raw8 {  // 16-bit types
 };
 template <>
 struct Raw8<float> {
-  float4 a, b;
+  uint4 a, b;
   __device__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    a = __ldg(reinterpret_cast<const uint4*>(p));
+    b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
   }
+  __device__ uint32_t max_bits(uint32_t m) const {
+    const uint32_t k = 0x7fffffffu;
+    const uint32_t x = max(max(a.x & k, a.y & k), max(a.z & k, a.w & k));
+    const uint32_t y = max(max(b.x & k, b.y & k), max(b.z & k, b.w & k));
+    return max(m, max(x, y));
+  }
+  __device__ static uint32_t one_bits(const float* p) {
+    return __ldg(reinterpret_cast<const uint32_t*>(p)) & 0x7fffffffu;
+  }
+  __device__ static float amax(uint32_t m) { return __uint_as_float(m); }
   __device__ void floats(float (&v)[8]) const {
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
   }
 };
 
 __device__ __forceinline__ float one_f32(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float one_f32(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float one_f32(const __half* p) { return __half2float(*p); }
-
-// Running |x| maximum that keeps NaN (fmaxf drops it): a row with NaN or infinity must show.
-__device__ __forceinline__ float amax_nan(float a, float x) {
-  x = fabsf(x);
-  return (x > a || x != x) ? x : a;
-}
 
 // The row's scale and 1 / scale: scale = max / 127 rounded once; 0 for a row whose scale is below 2^-120
 // (its codes are 0; q8_code's FMA would lose bits to underflow there), NaN for a row with NaN or
@@ -72,36 +87,64 @@ __device__ __forceinline__ void q8_scale(float amax, float& scale, float& inv) {
     inv = __frcp_rn(scale);
 }
 
-// Nearest integer to the real quotient x / scale, ties to even. x * inv is within 127 * 2^-22 of it, so
-// its rounding is right unless it lands within 1e-4 of a half; there the sign of x - half * scale, exact
-// from one FMA, decides.
-__device__ __forceinline__ int q8_code(float x, float scale, float inv) {
-  const float y = x * inv;
-  float k = rintf(y);
-  if (fabsf(y - k) > 0.4999f) {
-    const float lo = floorf(y);
-    const float r = fmaf(-(lo + 0.5f), scale, x);  // sign of x / scale - (lo + 1/2)
-    const float even = 2.0f * rintf(0.5f * (lo + 0.5f));
-    k = r > 0.0f ? lo + 1.0f : (r < 0.0f ? lo : even);
+// Nearest integers to the real quotients x / scale, ties to even, as 8-bit codes. y = x * inv is within
+// 127 * 2^-22 of the quotient, so rounding y is right unless it lies within 1e-4 of a half; there the sign of
+// x - half * scale, exact from one FMA, decides. Adding 1.5 * 2^23 rounds y and leaves its integer in the low
+// bits of the sum: no conversion instructions, of which the GPU issues a quarter as many per clock.
+constexpr float kRoundMagic = 12582912.0f;
+
+__device__ __forceinline__ uint32_t code_at_half(float x, float y, float scale) {
+  const float lo = floorf(y);
+  const float r = fmaf(-(lo + 0.5f), scale, x);  // sign of x / scale - (lo + 1/2)
+  const float even = 2.0f * rintf(0.5f * (lo + 0.5f));
+  const float k = r > 0.0f ? lo + 1.0f : (r < 0.0f ? lo : even);
+  return __float_as_uint(k + kRoundMagic);
+}
+
+// Rounded quotients as words whose low byte is the code; whether one of them lies next to a half.
+template <int N>
+__device__ __forceinline__ bool codes_of(const float (&v)[N], float inv, uint32_t (&k)[N]) {
+  bool near_half = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float y = v[j] * inv;
+    const float t = y + kRoundMagic;
+    k[j] = __float_as_uint(t);
+    near_half |= fabsf(y - (t - kRoundMagic)) > 0.4999f;
   }
-  return static_cast<int>(k);
+  return near_half;
 }
 
-__device__ __forceinline__ uint32_t pack4_i8(int a, int b, int c, int d) {
-  return (a & 0xFF) | ((b & 0xFF) << 8) | ((c & 0xFF) << 16) | (static_cast<uint32_t>(d) << 24);
+// The same where some quotient lies next to a half.
+template <int N>
+__device__ __forceinline__ void codes_at_halves(const float (&v)[N], float scale, float inv, uint32_t (&k)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float y = v[j] * inv;
+    const float t = y + kRoundMagic;
+    k[j] = fabsf(y - (t - kRoundMagic)) > 0.4999f ? code_at_half(v[j], y, scale) : __float_as_uint(t);
+  }
 }
 
-constexpr int kQ8Threads = 256;
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
-// A row belongs to kLanes threads (a warp, or the whole CTA). The row's first 8 * kLanes * kHeld values stay
-// in registers between the maximum and the codes, so such a row is read once, with all its loads in flight
-// together; what is longer is read again.
-template <typename T, int kLanes, int kHeld>
+constexpr int kQ8Threads = 128;
+constexpr int kQ8Held = 4;
+
+// A row belongs to kLanes threads (a warp, or the whole CTA). The row's first 32 * kLanes values stay in
+// registers between the maximum and the codes, so such a row is read once, with all its loads in flight
+// together; what is longer is read again. Vectors with a quotient next to a half are done a second time at the
+// end, out of line: bf16 rows have one in most rows, and the code for it unrolled into the main path made that
+// too long for the instruction cache (4096 rows of 4096: 23 us).
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(kQ8Threads)
     quantize_i8_kernel(const T* __restrict__ x, int64_t ld_x, int64_t rows, int64_t cols, int8_t* __restrict__ codes,
                        int64_t ld_codes, float* __restrict__ scale_out, int vec_ok) {
   grid_dep_launch();
-  __shared__ float red[kQ8Threads / 32];
+  __shared__ uint32_t red[kQ8Threads / 32];
   constexpr int kRows = kQ8Threads / kLanes;
   const int t = threadIdx.x % kLanes;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
@@ -109,62 +152,91 @@ __global__ void __launch_bounds__(kQ8Threads)
   const T* xr = x + row * ld_x;
   int8_t* cr = codes + row * ld_codes;
   const int64_t nv = vec_ok ? cols / 8 : 0;
-  Raw8<T> held[kHeld];
-  float v[8];
-  float amax = 0.0f;
+  Raw8<T> held[kQ8Held];
+  uint32_t bits = 0;
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h)
+  for (int h = 0; h < kQ8Held; ++h)
     if (t + h * kLanes < nv) held[h].load(xr + 8 * (t + h * kLanes));
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h) {
-    if (t + h * kLanes < nv) {
-      held[h].floats(v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = amax_nan(amax, v[j]);
-    }
-  }
-  for (int64_t i = t + kHeld * kLanes; i < nv; i += kLanes) {
+  for (int h = 0; h < kQ8Held; ++h)
+    if (t + h * kLanes < nv) bits = held[h].max_bits(bits);
+  for (int64_t i = t + kQ8Held * kLanes; i < nv; i += kLanes) {
     Raw8<T> r;
     r.load(xr + 8 * i);
-    r.floats(v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = amax_nan(amax, v[j]);
+    bits = r.max_bits(bits);
   }
-  for (int64_t i = 8 * nv + t; i < cols; i += kLanes) amax = amax_nan(amax, one_f32(xr + i));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = amax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float amax = Raw8<T>::amax(bits);
+  bits = 0;
+  for (int64_t i = 8 * nv + t; i < cols; i += kLanes) bits = max(bits, Raw8<T>::one_bits(xr + i));
+  // as bits again, now of the fp32 value: NaN stays on top
+  bits = max(__float_as_uint(amax), __float_as_uint(Raw8<T>::amax(bits)));
+  bits = __reduce_max_sync(0xffffffffu, bits);
   if (kLanes > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = bits;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kQ8Threads / 32; ++w) amax = amax_nan(amax, red[w]);
+    for (int w = 0; w < kQ8Threads / 32; ++w) bits = max(bits, red[w]);
   }
+  amax = __uint_as_float(bits);
   float scale, inv;
   q8_scale(amax, scale, inv);
   if (t == 0) scale_out[row] = scale;
   const bool live = inv != 0.0f;
-  auto put8 = [&](int64_t i) {
-    int k[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) k[j] = live ? q8_code(v[j], scale, inv) : 0;
-    *reinterpret_cast<uint2*>(cr + 8 * i) =
-        make_uint2(pack4_i8(k[0], k[1], k[2], k[3]), pack4_i8(k[4], k[5], k[6], k[7]));
+  auto store8 = [&](const uint32_t (&k)[8], int64_t i) {
+    const uint2 c = make_uint2(low_bytes(k[0], k[1], k[2], k[3]), low_bytes(k[4], k[5], k[6], k[7]));
+    *reinterpret_cast<uint2*>(cr + 8 * i) = live ? c : make_uint2(0, 0);
   };
+  auto put8 = [&](const Raw8<T>& r, int64_t i) {
+    float v[8];
+    uint32_t k[8];
+    r.floats(v);
+    const bool near_half = codes_of<8>(v, inv, k);
+    store8(k, i);
+    return near_half;
+  };
+  uint64_t halves = 0;  // bit h: this thread's vector h (of the first 64) has a quotient next to a half
 #pragma unroll
-  for (int h = 0; h < kHeld; ++h) {
-    if (t + h * kLanes < nv) {
-      held[h].floats(v);
-      put8(t + h * kLanes);
-    }
-  }
-  for (int64_t i = t + kHeld * kLanes; i < nv; i += kLanes) {
+  for (int h = 0; h < kQ8Held; ++h)
+    if (t + h * kLanes < nv && put8(held[h], t + h * kLanes)) halves |= 1ull << h;
+  int64_t from = nv;  // later ones are all done again
+#pragma unroll 1
+  for (int64_t i = t + kQ8Held * kLanes, h = kQ8Held; i < nv; i += kLanes, ++h) {
     Raw8<T> r;
     r.load(xr + 8 * i);
-    r.floats(v);
-    put8(i);
+    if (put8(r, i)) {
+      if (h < 64)
+        halves |= 1ull << h;
+      else
+        from = min(from, i);
+    }
   }
-  for (int64_t i = 8 * nv + t; i < cols; i += kLanes)
-    cr[i] = static_cast<int8_t>(live ? q8_code(one_f32(xr + i), scale, inv) : 0);
+#pragma unroll 1
+  for (;;) {
+    int64_t i;
+    if (halves != 0) {
+      i = t + static_cast<int64_t>(__ffsll(halves) - 1) * kLanes;
+      halves &= halves - 1;
+    } else if (from < nv) {
+      i = from;
+      from += kLanes;
+    } else {
+      break;
+    }
+    Raw8<T> r;
+    r.load(xr + 8 * i);
+    float v[8];
+    uint32_t k[8];
+    r.floats(v);
+    codes_at_halves<8>(v, scale, inv, k);
+    store8(k, i);
+  }
+#pragma unroll 1
+  for (int64_t i = 8 * nv + t; i < cols; i += kLanes) {
+    const float v[1] = {one_f32(xr + i)};
+    uint32_t k[1];
+    if (codes_of<1>(v, inv, k)) codes_at_halves<1>(v, scale, inv, k);
+    cr[i] = static_cast<int8_t>(live ? k[0] & 0xffu : 0u);
+  }
 }
 
 // ------------------------------------------------------------------------------------ epilogues
@@ -195,15 +267,12 @@ struct I8Out {
 };
 
 // Stores vocabulary entry j (this lane's) of the 32 tokens from r: 32 neighbouring outputs per warp and token,
-// coalesced rows without staging, whatever the output's alignment. s_scale: this warp's 32 floats of
-// shared memory, through which every lane gets the tokens' scales.
+// coalesced rows without staging, whatever the output's alignment. s_scale: the tokens' 32 scales in shared
+// memory, which every lane reads.
 template <typename OutT>
-__device__ __forceinline__ void store_tokens32(const I8Out& p, const float (&v)[32], float* s_scale, int j, int r,
-                                               float ws, float b, int lane) {
+__device__ __forceinline__ void store_tokens32(const I8Out& p, const float (&v)[32], const float* s_scale, int j, int r,
+                                               float ws, float b) {
   const int lim = p.rows - r;
-  __syncwarp();
-  s_scale[lane] = lane < lim ? ld_dep_f32(p.row_scale + r + lane) : 0.0f;
-  __syncwarp();
   OutT* dst = static_cast<OutT*>(p.out) + static_cast<int64_t>(r) * p.ld_out + j;
   const bool ok = j < p.cols;
   if (lim >= 32) {
@@ -227,48 +296,71 @@ __device__ __forceinline__ void store_tokens32(const I8Out& p, const float (&v)[
 }
 
 // Output tile of the plain product on the CTA-pair core. The weight is the A operand, so a thread owns one
-// vocabulary entry (TMEM lane).
+// vocabulary entry (TMEM lane); a warp has 128 of the tile's 256 tokens.
 template <typename OutT>
 struct Int8StoreEpilogue {
-  static constexpr int kSmemPerWarp = 128;
-  static constexpr int kSmemBytes = 8 * kSmemPerWarp;
+  static constexpr int kSmemBytes = 16 * 512;  // 128 scales per warp
   using Params = I8Out;
 
-  template <class Release>
-  __device__ __forceinline__ static void run(const Params& p, uint8_t* stage, uint32_t tacc, int m_blk, int n_blk,
-                                             int q, int lane, Release release) {
+  struct Tile {
+    float ws, b, xs[4];
+  };
+
+  __device__ __forceinline__ static Tile fetch(const Params& p, int m_blk, int n_blk, int half, int q, int lane) {
+    const int j = m_blk * kBM + q * 32 + lane;
+    const int r = n_blk * kBN + half * 128 + lane;
+    const bool ok = j < p.cols;
+    Tile t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.xs[i] = r + i * 32 < p.rows ? ld_dep_f32(p.row_scale + r + i * 32) : 0.0f;
+    t.ws = ok ? __ldg(p.col_scale + j) : 0.0f;
+    t.b = ok && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, j) : 0.0f;
+    return t;
+  }
+
+  __device__ __forceinline__ static void stage(const Tile& t, uint8_t* smem, int group, int half, int q, int lane) {
+    float* s_scale = reinterpret_cast<float*>(smem) + ((group * 2 + half) * 4 + q) * 128;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_scale[i * 32 + lane] = t.xs[i];
+    __syncwarp();
+  }
+
+  template <class Release, class Wait>
+  __device__ __forceinline__ static bool run(const Params& p, const Tile& tile, uint8_t* smem, uint32_t tacc, int m_blk,
+                                             int n_blk, int group, int half, int q, int lane, uint64_t* /*join*/,
+                                             uint32_t& /*joins*/, Release release, Wait /*wait*/) {
     const int j = m_blk * kBM + q * 32 + lane;  // vocabulary entry
-    const int r0 = n_blk * kBN;                 // first token
-    const int ntok = min(kBN, p.rows - r0);
+    const int r0 = n_blk * kBN + half * 128;    // first token
+    const int ntok = min(128, p.rows - r0);
+    const float* s_scale = reinterpret_cast<float*>(smem) + ((group * 2 + half) * 4 + q) * 128;
     if (j - lane < p.cols) {
-      const bool ok = j < p.cols;
-      const float ws = ok ? __ldg(p.col_scale + j) : 0.0f;
-      const float b = ok && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, j) : 0.0f;
       float v[32];
 #pragma unroll 1
       for (int c = 0; c < ntok; c += 32) {
         __syncwarp();
         tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
-        store_tokens32<OutT>(p, v, reinterpret_cast<float*>(stage), j, r0 + c, ws, b, lane);
+        store_tokens32<OutT>(p, v, s_scale + c, j, r0 + c, tile.ws, tile.b);
       }
     }
     release();
+    return true;
   }
 
   __device__ __forceinline__ static void finish(const Params&, int) {}
 };
 
-// Softmax partials of the scaled product, in one pass over the accumulator: thread = token (TMEM lane), 32
-// columns at a time with a running maximum, and s and u rescaled when it rises. Without a bias the token's
-// scale xs > 0 is taken out: with y = acc * wscale, z = xs y has its maximum where y has, exp(z - m) =
-// 2^((y - max y) xs log2 e), u = xs sum (y - max y) e. Pairs of columns share fp32x2 instructions; a column
-// costs about 6 issue slots, of which the conversion of its int32 and its exponential go to the
-// low-throughput unit.
-template <bool kBias>
+// Softmax partials of the scaled product, in one pass over the accumulator: thread = token (TMEM lane), 16
+// columns at a time with a running maximum, and s and u rescaled when it rises. A warp has 128 of the tile's
+// 256 columns; the two warps of a token join their statistics through shared memory. Pairs of columns share
+// fp32x2 instructions: a pair costs two int32 conversions, two exponentials, two maxima and five others.
+//   kFull = false: the token's scale xs >= 0 is taken out: with y = acc * wscale, z = xs y has its maximum where
+//     y has, exp(z - m) = 2^((y - max y) xs log2 e), u = xs sum (y - max y) e.
+//   kFull = true: z = (acc * wscale) * xs + bias, for a bias and for the caller's own scales (any sign).
+template <bool kFull>
 struct Int8CEPartialsEpilogue {
-  // 32 weight scales and 32 bias values of the current columns
-  static constexpr int kSmemPerWarp = 256;
-  static constexpr int kSmemBytes = 8 * kSmemPerWarp;
+  static constexpr int kJoinBytes = 8 * 32 * 16;  // (group, quarter) x 32 tokens
+  static constexpr int kSmemBytes = kJoinBytes + 16 * 1024;  // and 128 scales and 128 biases per warp
 
   struct Params {
     const float* row_scale;
@@ -284,116 +376,183 @@ struct Int8CEPartialsEpilogue {
     int* status;
   };
 
-  template <class Release>
-  __device__ __forceinline__ static void run(const Params& p, uint8_t* stage, uint32_t tacc, int m_blk, int n_blk,
-                                             int q, int lane, Release release) {
-    constexpr float kLow = -1e38f;  // below every logit; differences to it stay finite
+  struct Tile {
+    float xs, ws[4], b[kFull ? 4 : 1];
+    int tcol;  // the target's column among this warp's 128, if it is one of them
+  };
+
+  __device__ __forceinline__ static float* scales(uint8_t* smem, int group, int half, int q) {
+    return reinterpret_cast<float*>(smem + kJoinBytes) + ((group * 2 + half) * 4 + q) * 256;
+  }
+
+  __device__ __forceinline__ static Tile fetch(const Params& p, int m_blk, int n_blk, int half, int q, int lane) {
+    const int row = m_blk * kBM + q * 32 + lane;
+    const int n0 = n_blk * kBN + half * 128;
+    Tile t{};
+    t.tcol = -1;
+    if (row - lane >= p.rows) return t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int col = n0 + i * 32 + lane;
+      t.ws[i] = col < p.vocab_shard ? __ldg(p.col_scale + col) : 0.0f;
+      if (kFull) t.b[i] = col < p.vocab_shard && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, col) : 0.0f;
+    }
+    if (row < p.rows) {
+      t.xs = ld_dep_f32(p.row_scale + row);
+      const int64_t lt = p.target[row] - n0;
+      t.tcol = lt >= 0 && lt < min(128, p.vocab_shard - n0) ? static_cast<int>(lt) : -1;
+    }
+    return t;
+  }
+
+  __device__ __forceinline__ static void stage(const Tile& t, uint8_t* smem, int group, int half, int q, int lane) {
+    float* s_ws = scales(smem, group, half, q);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s_ws[i * 32 + lane] = t.ws[i];
+      if (kFull) s_ws[128 + i * 32 + lane] = t.b[i];
+    }
+    __syncwarp();
+  }
+
+  struct Stat {
+    float m, s, u, zt;
+  };
+
+  static constexpr float kLow = -1e38f;  // below every logit; differences to it stay finite
+
+  // 16 columns: r are their sums, s_ws their scales (and biases 128 behind them), `lim` of them valid; tcol the
+  // target's column among them, or -1.
+  template <bool kRagged>
+  __device__ __forceinline__ static void columns16(Stat& st, const uint32_t (&r)[16], const float* s_ws, int lim,
+                                                   uint64_t xs2, float k, uint64_t k2, int tcol) {
+    uint64_t y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(s_ws + 4 * i);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = 4 * i + 2 * h;
+        y[2 * i + h] = mul_f32x2(pack_f32x2(static_cast<float>(static_cast<int>(r[j])),
+                                            static_cast<float>(static_cast<int>(r[j + 1]))), h == 0 ? w.x : w.y);
+      }
+      if (kFull) {
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(s_ws + 128 + 4 * i);
+        y[2 * i] = fma_f32x2(y[2 * i], xs2, b.x);
+        y[2 * i + 1] = fma_f32x2(y[2 * i + 1], xs2, b.y);
+      }
+    }
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) unpack_f32x2(y[i], v[2 * i], v[2 * i + 1]);
+    if (kRagged) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j >= lim) v[j] = kLow;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+    }
+    if (tcol >= 0) st.zt = select16(v, tcol);
+    float t4[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t4[q] = fmaxf(fmaxf(v[4 * q], v[4 * q + 1]), fmaxf(v[4 * q + 2], v[4 * q + 3]));
+    const float top = fmaxf(st.m, fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])));
+    const float d = st.m - top;
+    const float e0 = ex2_approx(d * k);
+    const uint64_t neg = pack_f32x2(-top, -top);
+    uint64_t s2[2] = {0, 0}, u2[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t dd = add_f32x2(y[i], neg);
+      float a0, a1;
+      unpack_f32x2(mul_f32x2(dd, k2), a0, a1);
+      a0 = ex2_approx(a0);
+      a1 = ex2_approx(a1);
+      if (kRagged) {
+        a0 = 2 * i < lim ? a0 : 0.0f;
+        a1 = 2 * i + 1 < lim ? a1 : 0.0f;
+      }
+      const uint64_t e = pack_f32x2(a0, a1);
+      s2[i & 1] = add_f32x2(s2[i & 1], e);
+      u2[i & 1] = fma_f32x2(dd, e, u2[i & 1]);
+    }
+    st.u = fmaf(d, st.s, st.u) * e0;
+    st.s *= e0;
+    st.m = top;
+    float f0, f1;
+    unpack_f32x2(add_f32x2(s2[0], s2[1]), f0, f1);
+    st.s += f0 + f1;
+    unpack_f32x2(add_f32x2(u2[0], u2[1]), f0, f1);
+    st.u += f0 + f1;
+  }
+
+  template <class Release, class Wait>
+  __device__ __forceinline__ static bool run(const Params& p, const Tile& tile, uint8_t* smem, uint32_t tacc, int m_blk,
+                                             int n_blk, int group, int half, int q, int lane, uint64_t* join,
+                                             uint32_t& joins, Release release, Wait wait) {
     const int row0 = m_blk * kBM + q * 32;
     const int row = row0 + lane;
-    if (row0 >= p.rows) {
+    if (row0 >= p.rows) {  // both warps of these tokens
       release();
-      return;
+      return true;
     }
-    const int n0 = n_blk * kBN;
-    const int ncols = min(kBN, p.vocab_shard - n0);
+    const int n0 = n_blk * kBN + half * 128;
+    const int ncols = min(128, p.vocab_shard - n0);
     const bool row_ok = row < p.rows;
-    const float xs = row_ok ? ld_dep_f32(p.row_scale + row) : 0.0f;
-    // a negative scale (from the caller) turns the order round: then y = -acc * wscale with |xs|
-    const bool flip = !kBias && __any_sync(0xffffffffu, xs < 0.0f);
-    const float sign = xs < 0.0f ? -1.0f : 1.0f;
-    const float f = kBias ? 1.0f : fabsf(xs);
-    const float k = f * kLog2e;
+    const float* s_ws = scales(smem, group, half, q);
+    const float xs = tile.xs;
+    const float k = kFull ? kLog2e : xs * kLog2e;
     const uint64_t k2 = pack_f32x2(k, k), xs2 = pack_f32x2(xs, xs);
-    int tcol = -1;
-    if (row_ok && p.target != nullptr) {
-      const long long lt = static_cast<long long>(p.target[row]) - n0;
-      if (lt >= 0 && lt < ncols) tcol = static_cast<int>(lt);
-    }
-    float* s_ws = reinterpret_cast<float*>(stage);
-    float* s_b = s_ws + 32;
-    float ws = 0.0f, b = 0.0f;
-    auto fetch = [&](int c) {
-      const int col = c * 32 + lane;
-      ws = col < ncols ? __ldg(p.col_scale + n0 + col) : 0.0f;
-      if (kBias) b = col < ncols ? bias_at(p.bias, p.bias_dtype, n0 + col) : 0.0f;
-    };
-    fetch(0);
-    float v[32];
-    float m = kLow, zt = 0.0f, s = 0.0f, u = 0.0f;
+    const int tcol = tile.tcol;
+    Stat st = {kLow, 0.0f, 0.0f, 0.0f};
+    uint32_t r[16];
+    if (ncols == 128) {
 #pragma unroll 1
-    for (int c = 0; c * 32 < ncols; ++c) {
-      const int lim = ncols - c * 32;
-      __syncwarp();
-      s_ws[lane] = ws;
-      if (kBias) s_b[lane] = b;
-      __syncwarp();
-      if (lim > 32) fetch(c + 1);
-      tmem_load_32cols(tacc + static_cast<uint32_t>(c * 32), v);
-      uint64_t y[16];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(s_ws + 4 * i);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int j = 4 * i + 2 * h;
-          y[2 * i + h] = mul_f32x2(pack_f32x2(static_cast<float>(__float_as_int(v[j])),
-                                              static_cast<float>(__float_as_int(v[j + 1]))), h == 0 ? w.x : w.y);
-        }
-        if (kBias) {
-          const ulonglong2 bb = *reinterpret_cast<const ulonglong2*>(s_b + 4 * i);
-          y[2 * i] = fma_f32x2(y[2 * i], xs2, bb.x);
-          y[2 * i + 1] = fma_f32x2(y[2 * i + 1], xs2, bb.y);
-        }
+      for (int c = 0; c < 128; c += 16) {
+        __syncwarp();
+        tmem_load_16cols(tacc + static_cast<uint32_t>(c), r);
+        columns16<false>(st, r, s_ws + c, 16, xs2, k, k2, (tcol >> 4) == (c >> 4) ? tcol & 15 : -1);
       }
-      if (flip) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = mul_f32x2(y[i], pack_f32x2(sign, sign));
+    } else {
+#pragma unroll 1
+      for (int c = 0; c < ncols; c += 16) {
+        __syncwarp();
+        tmem_load_16cols(tacc + static_cast<uint32_t>(c), r);
+        columns16<true>(st, r, s_ws + c, ncols - c, xs2, k, k2, (tcol >> 4) == (c >> 4) ? tcol & 15 : -1);
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) unpack_f32x2(y[i], v[2 * i], v[2 * i + 1]);
-      if (lim < 32) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j >= lim) v[j] = kLow;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
-      }
-      if ((tcol >> 5) == c) zt = select32(v, tcol & 31);
-      float top = m;
-#pragma unroll
-      for (int j = 0; j < 32; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));
-      const float d = m - top;
-      const float r = ex2_approx(d * k);
-      u = fmaf(d, s, u) * r;
-      s *= r;
-      m = top;
-      const uint64_t neg = pack_f32x2(-top, -top);
-      uint64_t s2[2] = {0, 0}, u2[2] = {0, 0};
-      auto add = [&](int i, float live0, float live1) {
-        const uint64_t dd = add_f32x2(y[i], neg);
-        float a0, a1;
-        unpack_f32x2(mul_f32x2(dd, k2), a0, a1);
-        const uint64_t e = pack_f32x2(ex2_approx(a0) * live0, ex2_approx(a1) * live1);
-        s2[i & 1] = add_f32x2(s2[i & 1], e);
-        u2[i & 1] = fma_f32x2(dd, e, u2[i & 1]);
-      };
-      if (lim >= 32) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) add(i, 1.0f, 1.0f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) add(i, 2 * i < lim ? 1.0f : 0.0f, 2 * i + 1 < lim ? 1.0f : 0.0f);
-      }
-      float f0, f1;
-      unpack_f32x2(add_f32x2(s2[0], s2[1]), f0, f1);
-      s += f0 + f1;
-      unpack_f32x2(add_f32x2(u2[0], u2[1]), f0, f1);
-      u += f0 + f1;
     }
+    const float f = kFull ? 1.0f : xs;
+    st.m *= f;
+    st.u *= f;
+    st.zt *= f;
+    // The second half hands over through shared memory. The first gives the accumulator back only after it
+    // has read the slot, so the second cannot be at its next tile's write by then.
+    float4* slot = reinterpret_cast<float4*>(smem) + (group * 4 + q) * 32 + lane;
+    if (half == 1) {
+      *slot = make_float4(st.m, st.s, st.u, st.zt);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(join);
+      release();
+      return true;
+    }
+    const bool joined = wait(join, joins);
+    joins ^= 1u;
+    if (!joined) return false;
+    const float4 o = *slot;
     release();
-    if (row_ok && device_check(n_blk < p.n_tiles, p.status)) {
-      p.partials[static_cast<int64_t>(n_blk) * p.tile_stride + row] = make_float4(m * f, s, u * f, zt * f);
+    if (o.y != 0.0f) {  // the tile reaches into its second half
+      const float top = fmaxf(st.m, o.x);
+      const float d0 = st.m - top, d1 = o.x - top;
+      const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
+      st.u = fmaf(d0, st.s, st.u) * e0 + fmaf(d1, o.y, o.z) * e1;
+      st.s = st.s * e0 + o.y * e1;
+      st.m = top;
+      st.zt += o.w;
     }
+    if (row_ok && device_check(n_blk < p.n_tiles, p.status))
+      p.partials[static_cast<int64_t>(n_blk) * p.tile_stride + row] = make_float4(st.m, st.s, st.u, st.zt);
+    return true;
   }
 
   __device__ __forceinline__ static void finish(const Params&, int) {}
@@ -409,6 +568,7 @@ constexpr int kFewMaxTokens = 128;
 constexpr int kFewWBytes = 128 * 128;
 constexpr int kFewMaxStages = 6;
 constexpr int kFewRingBytes = 108 * 1024;
+constexpr int kFewOtherBytes = 1024 + 4 * 4 * kFewMaxTokens + 256;  // alignment, scales, barriers
 
 inline int few_tokens_padded(int64_t rows) { return static_cast<int>((rows + 15) / 16 * 16); }
 inline int few_stages(int nt) {
@@ -425,8 +585,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int x_bytes = nt * 128;
   uint8_t* s_w = smem;
   uint8_t* s_x = smem + stages * kFewWBytes;
-  float* s_scale = reinterpret_cast<float*>(s_x + stages * x_bytes);  // 32 per epilogue warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + 128);
+  float* s_scale = reinterpret_cast<float*>(s_x + stages * x_bytes);  // the tokens', per epilogue warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + 4 * kFewMaxTokens);
   uint64_t* empty = full + kFewMaxStages;
   uint64_t* done = empty + kFewMaxStages;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -519,6 +679,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const float ws = ok ? __ldg(p.col_scale + j) : 0.0f;
     const float b = ok && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, j) : 0.0f;
     grid_dep_wait();
+    float* s = s_scale + q * kFewMaxTokens;
+#pragma unroll
+    for (int i = 0; i < kFewMaxTokens; i += 32)
+      if (i < p.rows) s[i + lane] = i + lane < p.rows ? ld_dep_f32(p.row_scale + i + lane) : 0.0f;
+    __syncwarp();
     int good = 1;
     if (lane == 0)
       good = mbar_wait_bounded(done, 0, abort_flag, status, kStatusTimeoutEpilogue) && *abort_flag == 0 ? 1 : 0;
@@ -531,7 +696,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       for (int c = 0; c < p.rows; c += 32) {
         __syncwarp();
         tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
-        store_tokens32<OutT>(p, v, s_scale + q * 32, j, c, ws, b, lane);
+        store_tokens32<OutT>(p, v, s + c, j, c, ws, b);
       }
     }
   }
@@ -561,22 +726,19 @@ struct I8Operands {
 
 inline int64_t round_up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// Rows from which each row is left to one warp instead of one CTA. Measured on rows of 4096 bf16 values: see
-// frx_quantize_i8.
-constexpr int64_t kQ8WarpRows = 1024;
-
-template <typename T, int kHeldWarp>
+// Rows of up to 1024 values go to a warp each (16384 rows of 1024 bf16: see DESIGN), longer ones to a CTA.
+template <typename T>
 static int launch_quantize(const void* x, int64_t ld_x, int64_t rows, int64_t cols, int8_t* codes, int64_t ld_codes,
                            float* scale, cudaStream_t stream) {
   const int vec_ok = aligned16(x) && (ld_x * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7u) == 0 &&
                      ld_codes % 8 == 0;
   const T* xt = static_cast<const T*>(x);
-  if (rows >= kQ8WarpRows) {
+  if (cols <= 32 * 8 * kQ8Held) {
     constexpr int kRows = kQ8Threads / 32;
-    quantize_i8_kernel<T, 32, kHeldWarp><<<static_cast<unsigned>((rows + kRows - 1) / kRows), kQ8Threads, 0, stream>>>(
+    quantize_i8_kernel<T, 32><<<static_cast<unsigned>((rows + kRows - 1) / kRows), kQ8Threads, 0, stream>>>(
         xt, ld_x, rows, cols, codes, ld_codes, scale, vec_ok);
   } else {
-    quantize_i8_kernel<T, kQ8Threads, 4><<<static_cast<unsigned>(rows), kQ8Threads, 0, stream>>>(
+    quantize_i8_kernel<T, kQ8Threads><<<static_cast<unsigned>(rows), kQ8Threads, 0, stream>>>(
         xt, ld_x, rows, cols, codes, ld_codes, scale, vec_ok);
   }
   FRX_CUDA_CHECK(cudaGetLastError());
@@ -585,10 +747,10 @@ static int launch_quantize(const void* x, int64_t ld_x, int64_t rows, int64_t co
 
 static int quantize(const void* x, int dtype, int64_t ld_x, int64_t rows, int64_t cols, int8_t* codes,
                     int64_t ld_codes, float* scale, cudaStream_t stream) {
-  if (dtype == FRX_DTYPE_F32) return launch_quantize<float, 8>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
+  if (dtype == FRX_DTYPE_F32) return launch_quantize<float>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
   if (dtype == FRX_DTYPE_BF16)
-    return launch_quantize<__nv_bfloat16, 16>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
-  return launch_quantize<__half, 16>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
+    return launch_quantize<__nv_bfloat16>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
+  return launch_quantize<__half>(x, ld_x, rows, cols, codes, ld_codes, scale, stream);
 }
 
 // Checks shared by the two products; floating-point tokens are quantised into the workspace, whose used
@@ -653,18 +815,18 @@ static int launch_product(const I8Operands& op, void* out, int64_t ld_out, int* 
   if (rc) return rc;
   static std::atomic<uint64_t> attr_done{0};
   auto kernel = gemm_i8_few_kernel<OutT>;
-  constexpr int kMaxSmem = kFewRingBytes + 2048;
+  constexpr int kMaxSmem = kFewRingBytes + kFewOtherBytes;
   rc = ensure_smem_attr(kernel, attr_done, kMaxSmem);
   if (rc) return rc;
-  const int smem = stages * (kFewWBytes + nt * 128) + 2048;
+  const int smem = stages * (kFewWBytes + nt * 128) + kFewOtherBytes;
   return launch_kernel(kernel, static_cast<unsigned>((op.cols + 127) / 128), kFewThreads, smem, stream,
                        op.quantised_here, tm_w, tm_x, p, nt, static_cast<int>((op.k + 127) / 128), stages, status);
 }
 
-template <bool kBias>
+template <bool kFull>
 static int launch_score(const I8Operands& op, int64_t r0, int64_t n, const int64_t* target, float* partials,
                         int64_t tile_stride, int* status, cudaStream_t stream, bool overlap) {
-  using Epi = Int8CEPartialsEpilogue<kBias>;
+  using Epi = Int8CEPartialsEpilogue<kFull>;
   typename Epi::Params ep;
   memset(&ep, 0, sizeof(ep));
   ep.row_scale = op.x_scale + r0;
@@ -746,12 +908,13 @@ extern "C" int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t l
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const int64_t n = rows - r0 < step ? rows - r0 : step;
     const bool overlap = op.quantised_here && r0 == 0;
-    rc = bias != nullptr ? launch_score<true>(op, r0, n, target, partials, step, status, st, overlap)
-                         : launch_score<false>(op, r0, n, target, partials, step, status, st, overlap);
+    rc = bias != nullptr || !op.quantised_here
+             ? launch_score<true>(op, r0, n, target, partials, step, status, st, overlap)
+             : launch_score<false>(op, r0, n, target, partials, step, status, st, overlap);
     if (rc) return rc;
     auto at = [r0](float* p) { return p == nullptr ? nullptr : p + r0; };
-    rc = frx_finalize(partials, n_tiles, n, step, 0, target + r0, vocab_size, ignore_index, at(ce), at(entropy), at(lse),
-                      at(log_probs), nullptr, status, stream);
+    rc = launch_finalize_dep(partials, n_tiles, n, step, target + r0, vocab_size, ignore_index, at(ce), at(entropy),
+                             at(lse), at(log_probs), status, st);
     if (rc) return rc;
   }
   return FRX_OK;

@@ -114,16 +114,20 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t pa
 // Suspend-time hint of the pipeline waits: long enough that a waiting thread normally stays
 // parked until its phase completes, short enough to check the abort flag and deadline often.
 constexpr uint32_t kSuspendHintNs = 200000;
+// For the short pipelines of the 8-bit products (tiles of a few microseconds): 926 tokens x 3712 x 1265 took
+// 32 us with the long hint and 23 us with this one, larger products the same.
+constexpr uint32_t kSuspendHintShortNs = 1000;
 
 // Waits for the phase with the given parity. Returns false (and raises the abort flag and
 // the status bit) when the deadline passes, or returns false at once when another role has
 // already raised the abort flag.
 static __device__ __noinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                                int* status, int code, uint64_t limit_ns = kWaitLimitNs) {
+                                                int* status, int code, uint64_t limit_ns = kWaitLimitNs,
+                                                uint32_t suspend_ns = kSuspendHintNs) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_timer_ns();
   for (uint32_t n = 1;; ++n) {
-    if (mbar_try_wait_suspend(bar, parity, kSuspendHintNs)) return true;
+    if (mbar_try_wait_suspend(bar, parity, suspend_ns)) return true;
     if (*abort_flag) return false;
     if (global_timer_ns() - t0 > limit_ns) {
       *abort_flag = 1;
@@ -283,6 +287,23 @@ __device__ __forceinline__ void tmem_load_32cols(uint32_t taddr, float (&v)[32])
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same for 16 columns, as raw bits.
+__device__ __forceinline__ void tmem_load_16cols(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
 // ---------------------------------------------------------------------------------------
 // UMMA descriptors
 // ---------------------------------------------------------------------------------------
@@ -339,6 +360,13 @@ __device__ __forceinline__ void cluster_sync_all() {
 // Arrive on an mbarrier given by its shared::cluster address (possibly in the peer CTA).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// The same without cluster-scope release: for a phase that only hands over tensor memory, whose reads are
+// complete (tcgen05.wait::ld) and fenced before it. The cluster-scope release also waits for this thread's
+// global stores to be performed, about 1000 cycles after a tile's partials were stored.
+__device__ __forceinline__ void mbar_arrive_cluster_cta(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // TMA tile load into this CTA's shared memory whose completion is counted on an mbarrier that

@@ -19,12 +19,6 @@ from . import ops
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _vector(t: Tensor, name: str, n: int, dtype: torch.dtype) -> Tensor:
-    if t.dtype != dtype or t.shape != (n,):
-        raise ValueError(f"{name} must be {dtype} [{n}], got {t.dtype} {tuple(t.shape)}")
-    return t.contiguous()
-
-
 def _ids(t: Tensor, name: str) -> Tensor:
     if t.dim() != 1:
         raise ValueError(f"{name} must be 1-D, got shape {tuple(t.shape)}")
@@ -35,11 +29,11 @@ def _ids(t: Tensor, name: str) -> Tensor:
     return t.contiguous()
 
 
-def _rows(t: Tensor, name: str, n: int, vocab: Optional[int]) -> Tensor:
+def _rows(t: Tensor, name: str) -> Tensor:
     if t.dtype not in _FLOATS:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != n or (vocab is not None and t.shape[1] != vocab):
-        raise ValueError(f"{name} must be [{n}, {'V' if vocab is None else vocab}], got {tuple(t.shape)}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
@@ -76,30 +70,26 @@ def verify_drafts(
     emitted there and their log p_i (greedy: at temperature 1); -1 and 0 where nothing is emitted. A row that
     leaves nothing to draw emits -1 with log-probability -inf. Decisions are taken in 64 bits. No host
     synchronisation; nothing is differentiable."""
-    draft_tokens, cu_drafts = _ids(draft_tokens, "draft_tokens"), _ids(cu_drafts, "cu_drafts")
-    n, batch = draft_tokens.numel(), cu_drafts.numel() - 1
+    drafts, cu = _ids(draft_tokens, "draft_tokens"), _ids(cu_drafts, "cu_drafts")
+    n, batch = drafts.numel(), cu.numel() - 1
     if batch < 0:
         raise ValueError("cu_drafts must hold at least one offset")
-    if batch == 0 and n:
-        raise ValueError(f"{n} drafted tokens, but cu_drafts has no sequence")
-    logits = _rows(target_logits, "target_logits", n + batch, None)
-    vocab = logits.shape[1]
-    if vocab < 1:
-        raise ValueError("target_logits must have at least one column")
-    uniforms = _vector(uniforms, "uniforms", n, torch.float32)
-    final_uniforms = _vector(final_uniforms, "final_uniforms", batch, torch.float32)
+    logits = _rows(target_logits, "target_logits")
+    rows, vocab = logits.shape
+    if rows != n + batch or vocab < 1 or (batch == 0 and n):
+        raise ValueError(f"target_logits must have at least one column and a row for each of {n} drafts and {batch} "
+                         f"sequences, got {tuple(logits.shape)}")
     if draft_probs is not None:
-        draft_probs = _rows(draft_probs, "draft_probs", n, vocab)
+        draft_probs = _rows(draft_probs, "draft_probs")
     temps = None
     if isinstance(temperature, Tensor):
-        temps, temperature = _vector(temperature, "temperature", batch, torch.float32), 1.0
-    dev = ops._require_cuda(logits, draft_tokens, cu_drafts, uniforms, final_uniforms, draft_probs, temps)
+        temps, temperature = temperature.contiguous(), 1.0
+    dev = logits.device
     accepted = torch.empty(batch, device=dev, dtype=torch.int64)
-    tokens = torch.empty(n + batch, device=dev, dtype=torch.int64)
-    log_probs = torch.empty(n + batch, device=dev, dtype=torch.float32)
-    if batch:
-        chunks = (vocab + nat.FRX_VERIFY_CHUNK - 1) // nat.FRX_VERIFY_CHUNK
-        workspace = torch.empty((n + batch) * chunks * 4, device=dev, dtype=torch.float32)
-        ops.verify_drafts(logits, draft_tokens, cu_drafts, uniforms, final_uniforms, draft_probs, temps,
-                          float(temperature), workspace, accepted, tokens, log_probs)
+    tokens = torch.empty(rows, device=dev, dtype=torch.int64)
+    log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
+    workspace = torch.empty(4 * rows * ((vocab + nat.FRX_VERIFY_CHUNK - 1) // nat.FRX_VERIFY_CHUNK), device=dev,
+                            dtype=torch.float32)
+    ops.verify_drafts(logits, drafts, cu, uniforms.contiguous(), final_uniforms.contiguous(), draft_probs, temps,
+                      float(temperature), workspace, accepted, tokens, log_probs)
     return accepted, tokens, log_probs

@@ -30,7 +30,9 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _no_grad_inputs(*tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    for t in tensors:
+        if t is None or not t.requires_grad or not torch.is_grad_enabled():
+            continue
         raise NotImplementedError("the int8 head has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -79,7 +81,8 @@ def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
 
 def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: Optional[Tensor],
              hidden_scale: Optional[Tensor]):
-    """Checked operands: (hidden [M, H], hidden scale [M] or None, weight codes, weight scale, bias)."""
+    """Operands as the kernels read them, (hidden [M, H], hidden scale [M] or None, weight codes, weight scale, bias);
+    what does not concern the layout is checked at the launch (ops)."""
     if weight_codes.dim() != 2 or weight_codes.dtype != torch.int8:
         raise TypeError(f"weight_codes must be int8 [V, H], got {weight_codes.dtype} {tuple(weight_codes.shape)}")
     V, H = weight_codes.shape
@@ -87,30 +90,20 @@ def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: O
         raise ValueError(f"weight_codes must not be empty, got {tuple(weight_codes.shape)}")
     if H > nat.FRX_I8_MAX_K:
         raise NotImplementedError(f"hidden size {H} > {nat.FRX_I8_MAX_K} could overflow the int32 sums")
-    if hidden.dim() < 1 or hidden.shape[-1] != H:
+    dims = hidden.dim()
+    if dims < 1 or hidden.shape[-1] != H:
         raise ValueError(f"hidden size mismatch: hidden {tuple(hidden.shape)} vs weight_codes {tuple(weight_codes.shape)}")
-    if weight_scale.dtype != torch.float32 or weight_scale.shape != (V,):
-        raise ValueError(f"weight_scale must be float32 [{V}], got {weight_scale.dtype} {tuple(weight_scale.shape)}")
-    if bias is not None:
-        if bias.dtype not in _FLOATS or bias.shape != (V,):
-            raise ValueError(f"bias must be bfloat16, float16 or float32 [{V}], got {bias.dtype} {tuple(bias.shape)}")
-        bias = bias.contiguous()
-    if hidden.dtype == torch.int8:
-        if hidden_scale is None:
-            raise ValueError("int8 hidden states need hidden_scale (one float32 per token)")
-        if hidden_scale.dtype != torch.float32 or hidden_scale.shape != hidden.shape[:-1]:
+    _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
+    if hidden_scale is not None:
+        if hidden_scale.shape != hidden.shape[:-1]:
             raise ValueError(f"hidden_scale must be float32 {tuple(hidden.shape[:-1])}, got {hidden_scale.dtype} "
                              f"{tuple(hidden_scale.shape)}")
         hidden_scale = hidden_scale.reshape(-1).contiguous()
-    elif hidden.dtype not in _FLOATS:
-        raise TypeError(f"hidden must be bfloat16, float16, float32 or int8, got {hidden.dtype}")
-    elif hidden_scale is not None:
-        raise ValueError("hidden_scale goes with int8 hidden states; floating-point ones are quantised here")
-    _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
-    ops._require_cuda(hidden, weight_codes, weight_scale, bias, hidden_scale)
     x = _rows_2d(hidden)
     if hidden.dtype == torch.int8:
         x = _aligned_codes(x)
+    if bias is not None:
+        bias = bias.contiguous()
     return x, hidden_scale, _aligned_codes(weight_codes), weight_scale.contiguous(), bias
 
 
@@ -146,7 +139,8 @@ def int8_linear(
     x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
     rows, V = x.shape[0], w.shape[0]
     y = torch.empty(rows, V, device=x.device, dtype=out_dtype) if out is None else out
-    workspace = torch.empty(ops.i8_workspace_bytes(x), device=x.device, dtype=torch.uint8)
+    workspace = None if x_scale is not None else torch.empty(ops.i8_workspace_bytes(x), device=x.device,
+                                                             dtype=torch.uint8)
     ops.gemm_i8(x, x_scale, w, w_scale, y, workspace, bias=bias)
     return y if out is not None or hidden.dim() == 2 else y.view(*hidden.shape[:-1], V)
 

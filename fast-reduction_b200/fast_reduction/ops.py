@@ -473,15 +473,19 @@ def scale_inplace(x: torch.Tensor, scale: torch.Tensor) -> None:
     nat.check(rc, "frx_scale_inplace")
 
 
-# Device work of the functions below runs on the tensors' device whatever the current one is.
-def _launch_on(name: str, dev: torch.device, call) -> int:
-    if dev.index == torch.cuda.current_device():
-        return _launch(name, dev, call)
-    with torch.cuda.device(dev):
-        return _launch(name, dev, call)
-
-
 _I8_X_DTYPES = {**_OUT_DTYPES, torch.int8: nat.FRX_DTYPE_I8}
+
+
+def _call(name: str, entry: str, dev: torch.device, *args) -> None:
+    """One libfrx call on the tensors' device, whatever the current one is, with its status word and stream last."""
+    fn = getattr(nat.load(), entry)
+    if dev.index == torch.cuda.current_device():
+        rc = _launch(name, dev, lambda: fn(*args, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    else:
+        with torch.cuda.device(dev):
+            rc = _launch(name, dev, lambda: fn(*args, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+    if rc:
+        nat.check(rc, entry)
 
 
 def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
@@ -492,52 +496,61 @@ def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> No
     if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
         raise ValueError("codes must have x's shape and scale one value per row")
     lib = nat.load()
-    rc = _launch_on("quantize_i8", dev, lambda: lib.frx_quantize_i8(
-        x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
-        scale.data_ptr(), nat.stream_of(dev)))
+    with torch.cuda.device(dev):
+        rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
+            x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
+            scale.data_ptr(), nat.stream_of(dev)))
     nat.check(rc, "frx_quantize_i8")
 
 
 def i8_workspace_bytes(x: torch.Tensor) -> int:
     """Workspace of a product whose tokens are ``x`` [rows, k]: their codes and scales, unless they are codes."""
-    return 0 if x.dtype == torch.int8 else round_up(x.shape[0] * (round_up(x.shape[1], 16) + 4), 16)
+    rows, k = x.shape
+    return 0 if x.dtype == torch.int8 else (rows * ((k + 15) // 16 * 16 + 4) + 15) // 16 * 16
 
 
 def _i8_operands(x, x_scale, weight, weight_scale, bias):
-    """Checked operands of an 8-bit product: (device, the leading C arguments up to bias_dtype)."""
-    dev = _require_cuda(x, x_scale, weight, weight_scale, bias)
-    if x.dtype not in _I8_X_DTYPES or weight.dtype != torch.int8:
+    """Checked operands of an 8-bit product: (device, rows, cols, k, the leading C arguments up to bias_dtype)."""
+    xdt = _I8_X_DTYPES.get(x.dtype)
+    if xdt is None or weight.dtype != torch.int8:
         raise TypeError(f"x must be int8, bfloat16, float16 or float32 and weight int8, got {x.dtype} and {weight.dtype}")
-    ldx, ldw = _row_major(x, "x"), _row_major(weight, "weight")
     rows, k = x.shape
-    cols = weight.shape[0]
-    if weight.shape[1] != k:
+    cols, wk = weight.shape
+    if wk != k:
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
+    if x.stride(1) != 1 or weight.stride(1) != 1:
+        raise ValueError("x and weight must have unit column stride")
     if weight_scale.dtype != torch.float32 or weight_scale.shape != (cols,) or not weight_scale.is_contiguous():
-        raise ValueError(f"weight_scale must be contiguous float32 [{cols}]")
-    if (x_scale is None) != (x.dtype != torch.int8) or (x_scale is not None and (
-            x_scale.dtype != torch.float32 or x_scale.shape != (rows,) or not x_scale.is_contiguous())):
-        raise ValueError(f"x_scale must be contiguous float32 [{rows}] for int8 x, and None otherwise")
-    if bias is not None and (bias.dtype not in _OUT_DTYPES or bias.shape != (cols,) or not bias.is_contiguous()):
-        raise ValueError("bias must be a contiguous bfloat16, float16 or float32 vector with one value per weight row")
-    return dev, (x.data_ptr(), _I8_X_DTYPES[x.dtype], max(ldx, k), nat.ptr(x_scale), weight.data_ptr(), max(ldw, k),
-                 weight_scale.data_ptr(), nat.ptr(bias), 0 if bias is None else _OUT_DTYPES[bias.dtype])
+        raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
+                         f"{tuple(weight_scale.shape)}")
+    if x_scale is None:
+        if x.dtype == torch.int8:
+            raise ValueError("int8 tokens need their scales (hidden_scale)")
+    elif x.dtype != torch.int8 or x_scale.dtype != torch.float32 or x_scale.shape != (rows,) \
+            or not x_scale.is_contiguous():
+        raise ValueError(f"hidden_scale goes with int8 tokens, contiguous float32 [{rows}]")
+    bptr, bdt = None, 0
+    if bias is not None:
+        bdt = _OUT_DTYPES.get(bias.dtype)
+        if bdt is None or bias.shape != (cols,) or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous bfloat16, float16 or float32 [{cols}], got {bias.dtype} "
+                             f"{tuple(bias.shape)}")
+        bptr = bias.data_ptr()
+    dev = _require_cuda(x, x_scale, weight, weight_scale, bias)
+    return dev, rows, cols, k, (x.data_ptr(), xdt, max(x.stride(0), k), None if x_scale is None else x_scale.data_ptr(),
+                                weight.data_ptr(), max(weight.stride(0), k), weight_scale.data_ptr(), bptr, bdt)
 
 
 def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
             out: torch.Tensor, workspace: torch.Tensor | None, *, bias: torch.Tensor | None = None) -> None:
     """out[r, j] <- (xc[r] . weight[j]) * x_scale[r] * weight_scale[j] (+ bias[j]): xc = x for int8 x, else its codes,
     which go into the uint8 ``workspace`` (frx_gemm_i8)."""
-    dev, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
-    rows, cols = x.shape[0], weight.shape[0]
-    if out.dtype not in _OUT_DTYPES or out.shape != (rows, cols) or out.device != dev:
+    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
+    odt = _OUT_DTYPES.get(out.dtype)
+    if odt is None or out.shape != (rows, cols) or out.device != dev:
         raise ValueError(f"out must be bfloat16, float16 or float32 [{rows}, {cols}] on {dev}")
-    lib = nat.load()
-    rc = _launch_on("gemm_i8", dev, lambda: lib.frx_gemm_i8(
-        *operands, rows, cols, x.shape[1], nat.ptr(workspace), 0 if workspace is None else workspace.numel(),
-        out.data_ptr(), max(out.stride(0), cols), _OUT_DTYPES[out.dtype], nat.status_word(dev).data_ptr(),
-        nat.stream_of(dev)))
-    nat.check(rc, "frx_gemm_i8")
+    _call("gemm_i8", "frx_gemm_i8", dev, *operands, rows, cols, k, None if workspace is None else workspace.data_ptr(),
+          0 if workspace is None else workspace.numel(), out.data_ptr(), max(out.stride(0), cols), odt)
 
 
 def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -545,19 +558,15 @@ def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.T
                   workspace: torch.Tensor, *, launch_rows: int, ignore_index: int,
                   bias: torch.Tensor | None = None) -> None:
     """ce, entropy, log_probs <- those of gemm_i8's fp32 logits, launch_rows rows at a time (frx_i8_ce_entropy)."""
-    dev, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
-    rows = x.shape[0]
+    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
     if target.dtype != torch.int64 or not target.is_contiguous() or target.numel() != rows or target.device != dev:
-        raise ValueError("target must be a contiguous int64 tensor with one id per row")
-    for name, t in (("ce", ce), ("entropy", entropy), ("log_probs", log_probs)):
+        raise ValueError("target must be a contiguous int64 tensor with one id per row, on the tokens' device")
+    for t in (ce, entropy, log_probs):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != rows:
-            raise ValueError(f"{name} must be contiguous float32 with one value per row")
-    lib = nat.load()
-    rc = _launch_on("i8_ce_entropy", dev, lambda: lib.frx_i8_ce_entropy(
-        *operands, target.data_ptr(), rows, weight.shape[0], x.shape[1], ignore_index, launch_rows,
-        workspace.data_ptr(), workspace.numel(), ce.data_ptr(), entropy.data_ptr(), None, log_probs.data_ptr(),
-        nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
-    nat.check(rc, "frx_i8_ce_entropy")
+            raise ValueError("ce, entropy and log_probs must be contiguous float32 with one value per row")
+    _call("i8_ce_entropy", "frx_i8_ce_entropy", dev, *operands, target.data_ptr(), rows, cols, k, ignore_index,
+          launch_rows, workspace.data_ptr(), workspace.numel(), ce.data_ptr(), entropy.data_ptr(), None,
+          log_probs.data_ptr())
 
 
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor, uniforms: torch.Tensor,
@@ -565,31 +574,41 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
                   temperature_all: float, workspace: torch.Tensor, accepted: torch.Tensor, tokens: torch.Tensor,
                   log_probs: torch.Tensor) -> None:
     """accepted, tokens, log_probs <- the outcome of drafted tokens against target logits (frx_verify_drafts)."""
-    dev = _require_cuda(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature, workspace,
-                        accepted, tokens, log_probs)
     n, batch = drafts.numel(), cu_drafts.numel() - 1
-    if logits.dtype not in _LOGITS_DTYPES or (draft_probs is not None and draft_probs.dtype not in _LOGITS_DTYPES):
-        raise TypeError("logits and draft_probs must be bfloat16, float16 or float32")
-    ldl = max(_row_major(logits, "logits"), logits.shape[1])
+    dt = _LOGITS_DTYPES.get(logits.dtype)
+    if dt is None or logits.dim() != 2 or logits.shape[0] != n + batch or logits.stride(1) != 1:
+        raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V] with unit column stride, got "
+                         f"{logits.dtype} {tuple(logits.shape)} stride {logits.stride()}")
     vocab = logits.shape[1]
-    ldq = 0 if draft_probs is None else max(_row_major(draft_probs, "draft_probs"), vocab)
-    if logits.shape[0] != n + batch or (draft_probs is not None and draft_probs.shape != (n, vocab)):
-        raise ValueError("logits must have one row per draft and sequence, draft_probs one per draft")
-    for name, t, num, dt in (("drafts", drafts, n, torch.int64), ("cu_drafts", cu_drafts, batch + 1, torch.int64),
-                             ("uniforms", uniforms, n, torch.float32),
-                             ("final_uniforms", final_uniforms, batch, torch.float32),
-                             ("temperature", temperature, batch, torch.float32),
-                             ("accepted", accepted, batch, torch.int64), ("tokens", tokens, n + batch, torch.int64),
-                             ("log_probs", log_probs, n + batch, torch.float32)):
-        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() != num):
-            raise ValueError(f"{name} must be contiguous {dt} with {num} elements")
-    if workspace.dtype != torch.float32 or not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous float32")
-    lib = nat.load()
-    rc = _launch_on("verify_drafts", dev, lambda: lib.frx_verify_drafts(
-        logits.data_ptr(), _LOGITS_DTYPES[logits.dtype], ldl, drafts.data_ptr(), cu_drafts.data_ptr(),
-        uniforms.data_ptr(), final_uniforms.data_ptr(), nat.ptr(draft_probs),
-        0 if draft_probs is None else _LOGITS_DTYPES[draft_probs.dtype], ldq, nat.ptr(temperature),
-        temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
-        tokens.data_ptr(), log_probs.data_ptr(), nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
-    nat.check(rc, "frx_verify_drafts")
+    qptr, qdt, ldq = None, 0, 0
+    if draft_probs is not None:
+        qdt = _LOGITS_DTYPES.get(draft_probs.dtype)
+        if qdt is None or draft_probs.shape != (n, vocab) or draft_probs.stride(1) != 1:
+            raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}] with unit column stride, "
+                             f"got {draft_probs.dtype} {tuple(draft_probs.shape)} stride {draft_probs.stride()}")
+        qptr, ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
+    if drafts.dtype != torch.int64 or not drafts.is_contiguous():
+        raise ValueError("drafts must be contiguous int64")
+    if cu_drafts.dtype != torch.int64 or not cu_drafts.is_contiguous():
+        raise ValueError("cu_drafts must be contiguous int64")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (n,) or not uniforms.is_contiguous():
+        raise ValueError(f"uniforms must be contiguous float32 [{n}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+    if final_uniforms.dtype != torch.float32 or final_uniforms.shape != (batch,) or not final_uniforms.is_contiguous():
+        raise ValueError(f"final_uniforms must be contiguous float32 [{batch}], got {final_uniforms.dtype} "
+                         f"{tuple(final_uniforms.shape)}")
+    tptr = None
+    if temperature is not None:
+        if temperature.dtype != torch.float32 or temperature.shape != (batch,) or not temperature.is_contiguous():
+            raise ValueError(f"temperature must be contiguous float32 [{batch}], got {temperature.dtype} "
+                             f"{tuple(temperature.shape)}")
+        tptr = temperature.data_ptr()
+    dev = _require_cuda(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature)
+    for t, num, want in ((accepted, batch, torch.int64), (tokens, n + batch, torch.int64),
+                         (log_probs, n + batch, torch.float32)):
+        if t.dtype != want or not t.is_contiguous() or t.numel() != num or t.device != dev:
+            raise ValueError(f"outputs must be contiguous on {dev}: int64 accepted [{batch}], int64 tokens and float32 "
+                             f"log_probs [{n + batch}]")
+    _call("verify_drafts", "frx_verify_drafts", dev, logits.data_ptr(), dt, max(logits.stride(0), vocab),
+          drafts.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), final_uniforms.data_ptr(), qptr, qdt, ldq, tptr,
+          temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
+          tokens.data_ptr(), log_probs.data_ptr())

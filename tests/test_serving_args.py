@@ -76,7 +76,7 @@ def test_verify_entry_point():
 def test_int8_head_refusals():
     from fast_reduction import int8_ce_entropy, int8_linear, quantize_int8
 
-    x, w, s = torch.zeros(4, 32), torch.zeros(10, 32, dtype=torch.int8), torch.ones(10)
+    x, w, s = torch.zeros(4, 32), torch.zeros(10, 32, dtype=torch.int8), torch.ones(10)  # on the CPU
     t = torch.zeros(4, dtype=torch.int64)
     with pytest.raises(ValueError, match="CUDA"):
         quantize_int8(x)
@@ -141,7 +141,7 @@ def test_verify_refusals():
         call(cu_drafts=cu.float())
     with pytest.raises(ValueError, match="offset"):
         call(cu_drafts=cu[:0])
-    with pytest.raises(ValueError, match="no sequence"):
+    with pytest.raises(ValueError, match="0 sequences"):
         call(cu_drafts=cu[:1])
     with pytest.raises(ValueError, match="target_logits"):
         call(target_logits=z[:4])
