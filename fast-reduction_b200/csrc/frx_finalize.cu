@@ -51,10 +51,7 @@ constexpr int kFinSplits = 8;
 
 template <bool kDep>
 __device__ __forceinline__ float4 load_partial(const float4* p) {
-  if (!kDep) return __ldg(p);
-  float4 v;
-  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
-  return v;
+  return kDep ? ld_dep_v4(p) : __ldg(p);
 }
 
 // kDep: launched to overlap the end of the launch that wrote the partials (plain loads after the wait for it).

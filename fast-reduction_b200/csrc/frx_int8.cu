@@ -576,10 +576,92 @@ inline int few_stages(int nt) {
   return n < kFewMaxStages ? n : kFewMaxStages;
 }
 
+// Stores the product.
 template <typename OutT>
+struct FewStore {
+  using Params = I8Out;
+  __device__ __forceinline__ static const I8Out& operands(const Params& p) { return p; }
+
+  __device__ __forceinline__ static void run(const Params& p, bool good, uint8_t* /*ring*/, const float* s_scale,
+                                             uint32_t tacc, int n0, int q, int lane, float ws, float b, int* /*status*/) {
+    const int j = n0 + q * 32 + lane;
+    if (!good || j - lane >= p.cols) return;
+    float v[32];
+#pragma unroll 1
+    for (int c = 0; c < p.rows; c += 32) {
+      __syncwarp();
+      tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
+      store_tokens32<OutT>(p, v, s_scale + c, j, c, ws, b);
+    }
+  }
+};
+
+// Reduces the product to softmax partials of 128 columns: the logits go to shared memory (the ring, which is free by
+// then), [token][column], and 128 / tokens threads (a power of two, at most 32) take a token each way.
+struct FewScore {
+  struct Params {
+    I8Out op;  // no output
+    const int64_t* target;
+    float4* partials;
+    int64_t tile_stride;
+    int n_tiles;
+  };
+  __device__ __forceinline__ static const I8Out& operands(const Params& p) { return p.op; }
+
+  __device__ __forceinline__ static void run(const Params& p, bool good, uint8_t* ring, const float* s_scale,
+                                             uint32_t tacc, int n0, int q, int lane, float ws, float b, int* status) {
+    const int rows = p.op.rows;
+    const int tid = q * 32 + lane;
+    int parts = 32;
+    while (parts * rows > 128) parts >>= 1;
+    const int pitch = 128 + parts;  // lanes of a warp fall on different banks
+    float* zbuf = reinterpret_cast<float*>(ring);
+    if (good) {
+      float v[32];
+#pragma unroll 1
+      for (int c = 0; c < rows; c += 32) {
+        __syncwarp();
+        tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (c + i < rows)
+            zbuf[(c + i) * pitch + tid] = fmaf(static_cast<float>(__float_as_int(v[i])) * s_scale[c + i], ws, b);
+      }
+    }
+    // all four warps come here, whatever their waits said
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (!good) return;
+    const int token = tid / parts, part = tid % parts;
+    const int ncols = min(128, p.op.cols - n0);
+    const float* z = zbuf + (token < rows ? token : 0) * pitch;
+    float m = -INFINITY;
+    for (int j = part; j < ncols; j += parts) m = fmaxf(m, z[j]);
+    for (int o = 1; o < parts; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s = 0.0f, u = 0.0f;
+    for (int j = part; j < ncols; j += parts) {
+      const float d = z[j] - m;
+      const float e = ex2_approx(d * kLog2e);
+      s += e;
+      u = fmaf(d, e, u);
+    }
+    for (int o = 1; o < parts; o <<= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    const int tile = n0 >> 7;
+    if (token < rows && part == 0 && device_check(tile < p.n_tiles, status)) {
+      const int64_t t = p.target[token] - n0;
+      p.partials[tile * p.tile_stride + token] = make_float4(m, s, u, t >= 0 && t < ncols ? z[t] : 0.0f);
+    }
+  }
+};
+
+template <class Epi>
 __global__ void __launch_bounds__(kFewThreads, 2)
     gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                       const __grid_constant__ I8Out p, int nt, int num_k, int stages, int* status) {
+                       const __grid_constant__ typename Epi::Params ep, int nt, int num_k, int stages, int* status) {
+  const I8Out& p = Epi::operands(ep);
+  grid_dep_launch();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int x_bytes = nt * 128;
@@ -688,17 +770,8 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (lane == 0)
       good = mbar_wait_bounded(done, 0, abort_flag, status, kStatusTimeoutEpilogue) && *abort_flag == 0 ? 1 : 0;
     good = __shfl_sync(0xffffffffu, good, 0);
-    if (good && j - lane < p.cols) {
-      tc_fence_after();
-      const uint32_t tacc = tmem + (static_cast<uint32_t>(q * 32) << 16);
-      float v[32];
-#pragma unroll 1
-      for (int c = 0; c < p.rows; c += 32) {
-        __syncwarp();
-        tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
-        store_tokens32<OutT>(p, v, s + c, j, c, ws, b);
-      }
-    }
+    tc_fence_after();
+    Epi::run(ep, good != 0, s_w, s, tmem + (static_cast<uint32_t>(q * 32) << 16), n0, q, lane, ws, b, status);
   }
   tc_fence_before();
   __syncthreads();
@@ -799,13 +872,8 @@ static int prepare_i8(const char* what, const void* x, int x_dtype, int64_t ld_x
   return FRX_OK;
 }
 
-template <typename OutT>
-static int launch_product(const I8Operands& op, void* out, int64_t ld_out, int* status, cudaStream_t stream) {
-  I8Out p = {op.x_scale, op.w_scale, op.bias, op.bias_dtype, out, ld_out, static_cast<int>(op.rows),
-             static_cast<int>(op.cols)};
-  if (op.rows > kFewMaxTokens)
-    return launch_gemm_i8<Int8StoreEpilogue<OutT>>(op.w, op.ld_w, op.x, op.ld_x, op.cols, op.rows, op.k, 16, p, status,
-                                                   stream, op.quantised_here);
+template <class Epi>
+static int launch_few(const I8Operands& op, const typename Epi::Params& ep, int* status, cudaStream_t stream) {
   const int nt = few_tokens_padded(op.rows);
   const int stages = few_stages(nt);
   CUtensorMap tm_w, tm_x;
@@ -814,13 +882,35 @@ static int launch_product(const I8Operands& op, void* out, int64_t ld_out, int* 
   rc = encode_8bit_2d(&tm_x, op.x, op.rows, op.k, op.ld_x, nt, 128);
   if (rc) return rc;
   static std::atomic<uint64_t> attr_done{0};
-  auto kernel = gemm_i8_few_kernel<OutT>;
+  auto kernel = gemm_i8_few_kernel<Epi>;
   constexpr int kMaxSmem = kFewRingBytes + kFewOtherBytes;
   rc = ensure_smem_attr(kernel, attr_done, kMaxSmem);
   if (rc) return rc;
   const int smem = stages * (kFewWBytes + nt * 128) + kFewOtherBytes;
   return launch_kernel(kernel, static_cast<unsigned>((op.cols + 127) / 128), kFewThreads, smem, stream,
-                       op.quantised_here, tm_w, tm_x, p, nt, static_cast<int>((op.k + 127) / 128), stages, status);
+                       op.quantised_here, tm_w, tm_x, ep, nt, static_cast<int>((op.k + 127) / 128), stages, status);
+}
+
+template <typename OutT>
+static int launch_product(const I8Operands& op, void* out, int64_t ld_out, int* status, cudaStream_t stream) {
+  const I8Out p = {op.x_scale, op.w_scale, op.bias, op.bias_dtype, out, ld_out, static_cast<int>(op.rows),
+                   static_cast<int>(op.cols)};
+  if (op.rows <= kFewMaxTokens) return launch_few<FewStore<OutT>>(op, p, status, stream);
+  return launch_gemm_i8<Int8StoreEpilogue<OutT>>(op.w, op.ld_w, op.x, op.ld_x, op.cols, op.rows, op.k, 16, p, status,
+                                                 stream, op.quantised_here);
+}
+
+// Softmax partials of up to kFewMaxTokens tokens, one per 128 columns.
+static int launch_few_score(const I8Operands& op, const int64_t* target, float* partials, int64_t n_tiles, int* status,
+                            cudaStream_t stream) {
+  FewScore::Params ep = {};
+  ep.op = {op.x_scale, op.w_scale, op.bias, op.bias_dtype, nullptr, 0, static_cast<int>(op.rows),
+           static_cast<int>(op.cols)};
+  ep.target = target;
+  ep.partials = reinterpret_cast<float4*>(partials);
+  ep.tile_stride = op.rows;
+  ep.n_tiles = static_cast<int>(n_tiles);
+  return launch_few<FewScore>(op, ep, status, stream);
 }
 
 template <bool kFull>
@@ -895,8 +985,11 @@ extern "C" int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t l
   FRX_REQUIRE(rows <= 0 || (launch_rows >= 1 && target != nullptr), FRX_ERR_INVALID_ARG,
               "frx_i8_ce_entropy: need targets and launch_rows >= 1 (got %lld)", (long long)launch_rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t n_tiles = vocab_size > 0 ? (vocab_size + kBN - 1) / kBN : 0;
-  const int64_t step = launch_rows < rows ? launch_rows : rows;
+  // Few tokens go in one launch, whose partials cover 128 columns, whatever launch_rows is.
+  const bool few = rows <= kFewMaxTokens;
+  const int64_t tile = few ? 128 : kBN;
+  const int64_t n_tiles = vocab_size > 0 ? (vocab_size + tile - 1) / tile : 0;
+  const int64_t step = few || launch_rows >= rows ? rows : launch_rows;
   FRX_CHECK_RANGE(target, rows * 8, "frx_i8_ce_entropy: target");
   I8Operands op;
   int64_t used = 0;
@@ -908,7 +1001,8 @@ extern "C" int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t l
   for (int64_t r0 = 0; r0 < rows; r0 += step) {
     const int64_t n = rows - r0 < step ? rows - r0 : step;
     const bool overlap = op.quantised_here && r0 == 0;
-    rc = bias != nullptr || !op.quantised_here
+    rc = few ? launch_few_score(op, target, partials, n_tiles, status, st)
+         : bias != nullptr || !op.quantised_here
              ? launch_score<true>(op, r0, n, target, partials, step, status, st, overlap)
              : launch_score<false>(op, r0, n, target, partials, step, status, st, overlap);
     if (rc) return rc;

@@ -346,6 +346,12 @@ __device__ __forceinline__ uint32_t cluster_cta_rank() {
   return r;
 }
 
+__device__ __forceinline__ uint32_t cluster_cta_count() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
 // shared::cluster address of the variable at local address `saddr` in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t rank) {
   uint32_t r;
@@ -442,9 +448,17 @@ __device__ __forceinline__ void umma_commit_pair_mc(uint64_t* bar, uint16_t cta_
 // Lets the dependent grid start (once every CTA of this one has called it or ended).
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // Waits until the predecessor has ended and its writes are visible. What it wrote is then read with
-// ld_dep_f32 or through TMA, not with __ldg, whose loads the compiler may move up across the wait.
+// ld_dep_f32, ld_dep_v4 or through TMA, not with __ldg, whose loads the compiler may move up across the wait.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+__device__ __forceinline__ float4 ld_dep_v4(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ float ld_dep_f32(const float* p) {
   float v;
   asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");

@@ -10,33 +10,41 @@
 //     w = p_n                 when all were accepted,
 //   as the first j with w_j > 0 and  sum_{k <= j} w_k > r sum_k w_k.
 // T < 1e-6 (or NaN) is greedy: d_i is accepted while it equals argmax z_i (lowest index of a tie), and
-// the next token is the argmax. NaN logits count as -inf, +inf as the largest float, negative or NaN
+// the next token is the argmax. NaN logits count as -inf, +inf as the largest finite one, negative or NaN
 // draft probabilities as 0.
 //
 // Two launches:
-//   stats   one warp per (row, 2048 columns): max, sum of exp((z - max) / T) and the index of the max.
+//   stats   one warp per (row, 2048 or more columns): max, sum of exp((z - max) / T) and the index of the max.
 //           Reads every logit once: HBM-bound.
-//   sample  one cluster of 8 CTAs per sequence: merges the row statistics, decides a, then draws from
+//   sample  one cluster of 1 to 8 CTAs per sequence: merges the row statistics, decides a, then draws from
 //           the chosen row. Running sums and probabilities are in 64 bits: which token's interval a
 //           number falls in is a comparison over up to V borders, and sums in 32 bits would move each
-//           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256.
+//           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256. It is
+//           bound by issue slots and the 64-bit pipe (64 lanes per SM and clock), so the exponential is a
+//           short one of its own (exp2_scaled below).
 #include <cmath>
+#include <type_traits>
 
 #include "frx_epilogue.cuh"
 #include "frx_host.cuh"
 
 namespace frx {
 
-constexpr int kVfyChunk = 2048;  // columns per statistics partial
+constexpr int kVfyChunk = 2048;  // least columns per statistics partial (up to 7 of a first one lie before the row)
 constexpr int kVfyThreads = 256;
 constexpr int kVfyWarps = kVfyThreads / 32;
-constexpr int kVfyCluster = 8;
+constexpr int kVfyMaxCluster = 8;
+constexpr int kVfyMaxGroups = 16;  // groups of columns per warp whose lane sums are kept for the search
 constexpr float kVfyMinTemp = 1e-6f;
 constexpr float kVfyMaxTemp = 1e6f;
 constexpr float kFltMax = 3.402823466e38f;
 
-// NaN counts as masked, +inf as the largest finite value (so that differences stay numbers).
-__device__ __forceinline__ float clean_logit(float z) { return z == z ? fminf(z, kFltMax) : -INFINITY; }
+// NaN counts as masked (fmaxf drops it), +inf as a finite value no other logit exceeds (so that differences stay
+// numbers): the largest float, or for 16-bit logits the largest bf16 value, whose low 16 bits are zero.
+template <typename T>
+__device__ __forceinline__ float clean_logit(float z) {
+  return fminf(fmaxf(z, -INFINITY), sizeof(T) == 4 ? kFltMax : 3.38953139e38f);
+}
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T x);
@@ -47,30 +55,100 @@ __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return
 template <>
 __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
 
-// Eight consecutive values as floats (16-byte aligned when vec).
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int64_t n_valid, float fill, float (&v)[8]) {
-  if (vec && n_valid >= 8) {
-    if (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2(w[i], std::is_same<T, __half>::value);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n_valid ? to_f32<T>(p[i]) : fill;
+// 2^(j / 1024) = coarse[j / 32] * fine[j % 32], rounded to 64 bits each.
+struct Exp2Table {
+  double coarse[32], fine[32];
+};
+static Exp2Table make_exp2_table() {
+  Exp2Table t;
+  for (int j = 0; j < 32; ++j) {
+    t.coarse[j] = static_cast<double>(exp2l(static_cast<long double>(j) / 32.0L));
+    t.fine[j] = static_cast<double>(exp2l(static_cast<long double>(j) / 1024.0L));
   }
+  return t;
 }
+constexpr int kExp2Entries = 1024;
+
+// scale * 2^(a b / 1024) for -1024 * 1000 <= a b < 1024, table[j] = scale * 2^(j / 1024): by table and polynomial
+// (P. T. P. Tang, "Table-driven implementation of the exponential function in IEEE floating-point
+// arithmetic", 1989). a b = 1024 n + j + f with |f| <= 1/2; 2^(f / 1024) = e^x with |x| <= h = ln 2 / 2048 as
+// 1 + (1 + h^2 / 8) x + x^2 / 2, the Taylor terms with the cubic one economised (Lanczos: x^3 is (3/4) h^2 x to
+// within h^3 / 4 there), which is 1.6e-12 off at most and odd in x, so that sums over many values gain more.
+// Adding 1.5 * 2^52 rounds to an integer. Seven 64-bit operations; a table of 64 entries took four more.
+// Outside the range the result is some number, which the caller drops.
+__device__ __forceinline__ double exp2_scaled(double a, double b, const double* table) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
+  constexpr double kLn = 0.6931471805599453094 / kExp2Entries;
+  constexpr double c1 = kLn * (1.0 + kLn * kLn / 32), c2 = kLn * kLn / 2;  // h = kLn / 2
+  const double r = fma(a, b, kMagic);
+  const int k = __double2loint(r);
+  const double f = fma(a, b, kMagic - r);
+  const double g = f * fma(f, c2, c1);
+  const double t = table[k & (kExp2Entries - 1)];
+  // times 2^(k >> 10) through the exponent field
+  const double s = __hiloint2double((k & ~(kExp2Entries - 1)) * (1 << 10) + __double2hiint(t), __double2loint(t));
+  return fma(s, g, s);
+}
+
+// An fp32 value in 64 bits by its bits (conversions run at a quarter of the 64-bit pipe's rate). Zero and
+// subnormals come out as up to 2^-126 instead, which no logit notices. T: the type the value was read as (the
+// low word is zero for the 16-bit ones).
+template <typename T>
+__device__ __forceinline__ double widen(float x) {
+  const int b = __float_as_int(x);
+  return __hiloint2double(((b >> 3) & 0x8fffffff) + (896 << 20), sizeof(T) == 4 ? b << 29 : 0);
+}
+
+// The same for a draft probability, with negative values, NaN and subnormals as 0 (infinity: above every
+// probability).
+template <typename T>
+__device__ __forceinline__ double widen_prob(float x) {
+  const int b = __float_as_int(fmaxf(x, 0.0f));
+  return __hiloint2double(b >= 0x800000 ? (b >> 3) + (896 << 20) : 0, sizeof(T) == 4 ? b << 29 : 0);
+}
+
+// Eight values of a row as they lie in memory (two per word for 16-bit types).
+template <typename T>
+struct Vec8 {
+  static constexpr int kWords = sizeof(T) == 4 ? 8 : 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {  // 16-byte aligned
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    if (sizeof(T) == 4) {
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+      w[kWords - 4] = b.x; w[kWords - 3] = b.y; w[kWords - 2] = b.z; w[kWords - 1] = b.w;
+    }
+  }
+  // Values p[j * step] for the j with lo <= j * step < hi; `fill` (bits of a T) for the others.
+  __device__ __forceinline__ void load_some(const T* p, int step, int lo, int hi, uint32_t fill) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t x = fill;
+      if (j * step >= lo && j * step < hi)
+        x = sizeof(T) == 4 ? __ldg(reinterpret_cast<const uint32_t*>(p) + j * step)
+                           : __ldg(reinterpret_cast<const uint16_t*>(p) + j * step);
+      if (sizeof(T) == 4)
+        w[j % kWords] = x;
+      else
+        w[j / 2] = (j & 1) ? (w[j / 2] | (x << 16)) : x;
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[j % kWords]);
+    const float2 f = unpack2(w[j / 2], std::is_same<T, __half>::value);
+    return (j & 1) ? f.y : f.x;
+  }
+  __device__ __forceinline__ void mask(int j) {  // value j becomes -inf
+    if (sizeof(T) == 4)
+      w[j % kWords] = kNegInf;
+    else
+      w[j / 2] = (j & 1) ? ((w[j / 2] & 0xffffu) | (kNegInf << 16)) : ((w[j / 2] & 0xffff0000u) | kNegInf);
+  }
+  static constexpr uint32_t kNegInf =
+      sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00u : 0xff80u);
+};
 
 struct VerifyArgs {
   const void* logits;
@@ -94,6 +172,10 @@ struct VerifyArgs {
   int64_t* tokens;
   float* log_probs;
   int* status;
+  int chunk_cols;  // columns per statistics partial: kVfyChunk times a power of two
+  int row_step;    // stats: rows of a sequence are dealt to this many blocks
+  int strip_step;  // sample: 256-column strips per group of columns
+  Exp2Table exp2;
 };
 
 struct SeqTemp {
@@ -112,96 +194,153 @@ __device__ __forceinline__ SeqTemp seq_temp(const VerifyArgs& a, int64_t b) {
 // Offsets as the kernels use them: clamped into the draft array whatever the caller passed.
 __device__ __forceinline__ int64_t clamp_offset(int64_t x, int64_t n) { return x < 0 ? 0 : (x > n ? n : x); }
 
-// Sequence that owns logits row `row`: the last b with cu[b] + b <= row.
-__device__ __forceinline__ int64_t row_owner(const VerifyArgs& a, int64_t row) {
-  int64_t lo = 0, hi = a.batch - 1;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (clamp_offset(__ldg(a.cu + mid), a.n_drafts) + mid <= row)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kVfyThreads) verify_stats_kernel(VerifyArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = a.n_drafts + a.batch;
-  const int64_t units = rows * a.n_chunks;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kVfyWarps + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const int64_t row = unit / a.n_chunks;
-  const int chunk = static_cast<int>(unit - row * a.n_chunks);
-  // rows behind the last sequence's are not read
-  if (row >= clamp_offset(__ldg(a.cu + a.batch), a.n_drafts) + a.batch) return;
-  const SeqTemp st = seq_temp(a, row_owner(a, row));
-  const int64_t c0 = static_cast<int64_t>(chunk) * kVfyChunk;
-  const int64_t n = min(static_cast<int64_t>(kVfyChunk), a.vocab - c0);
-  const T* z = static_cast<const T*>(a.logits) + row * a.ld_logits + c0;
-  constexpr int kIter = kVfyChunk / 256;
-  float v[kIter][8];
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int64_t c = i * 256 + lane * 8;
-    load8<T>(z + c, a.logits_vec != 0, n - c, -INFINITY, v[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < kIter; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[i][j] = clean_logit(v[i][j]);
-      m = fmaxf(m, v[i][j]);
-    }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float s = 0.0f;
-  uint32_t idx = 0xFFFFFFFFu;
-  if (m > -INFINITY) {
-    const float k = kLog2e / st.t;
-#pragma unroll
-    for (int i = 0; i < kIter; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += ex2_approx((v[i][j] - m) * k);
-    if (st.greedy) {
-#pragma unroll
-      for (int i = 0; i < kIter; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (v[i][j] == m) idx = min(idx, static_cast<uint32_t>(c0 + i * 256 + lane * 8 + j));
-      idx = __reduce_min_sync(0xffffffffu, idx);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  }
-  if (lane == 0) a.partials[row * a.n_chunks + chunk] = make_float4(m, s, __uint_as_float(idx), 0.0f);
-}
-
-// Statistics of one whole row, the same in every lane.
+// The running maximum (from -FLT_MAX), sum of exp((z - m) / T) and index of the maximum of one lane or row; s = 0
+// says that nothing but masked logits was seen.
 struct RowStats {
   float m;
-  double s;
+  float s;
   uint32_t idx;
 };
 
+__device__ __forceinline__ void join_stats(RowStats& r, const RowStats& o, float k) {
+  const float m = fmaxf(r.m, o.m);
+  // the lowest index of a tie; a side without a live logit has none
+  if (o.s > 0.0f && (r.s == 0.0f || o.m > r.m || (o.m == r.m && o.idx < r.idx))) r.idx = o.idx;
+  r.s = r.s * ex2_approx((r.m - m) * k) + o.s * ex2_approx((o.m - m) * k);
+  r.m = m;
+}
+
+// Adds 8 N values to a lane's statistics: those of N vectors 256 columns apart, the first one's column is col.
+template <typename T, int N>
+__device__ __forceinline__ void add_vectors(RowStats& r, const Vec8<T> (&raw)[N], float k, bool greedy, uint32_t col) {
+  float v[8 * N], top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 8 * N; ++j) v[j] = raw[j / 8].at(j % 8);
+#pragma unroll
+  for (int j = 0; j < 8 * N; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));  // drops NaN
+  float sum;
+  auto add = [&]() {
+    if (greedy && (top > r.m || (r.s == 0.0f && top == r.m))) {
+#pragma unroll
+      for (int j = 8 * N - 1; j >= 0; --j)
+        if (v[j] == top) r.idx = col + (j / 8) * 256 + j % 8;
+    }
+    const float m = fmaxf(r.m, top), was = r.s * ex2_approx((r.m - m) * k);
+    const uint64_t neg = pack_f32x2(-m, -m), k2 = pack_f32x2(k, k);
+    uint64_t s2 = 0, s3 = 0;
+#pragma unroll
+    for (int j = 0; j < 8 * N; j += 2) {
+      float a0, a1;
+      unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(v[j], v[j + 1]), neg), k2), a0, a1);
+      const uint64_t e = pack_f32x2(ex2_approx(a0), ex2_approx(a1));
+      if (j & 2)
+        s3 = add_f32x2(s3, e);
+      else
+        s2 = add_f32x2(s2, e);
+    }
+    float f0, f1;
+    unpack_f32x2(add_f32x2(s2, s3), f0, f1);
+    sum = f0 + f1;
+    if (sum <= 8.5f * N) {
+      r.s = was + sum;
+      r.m = m;
+    }
+  };
+  // No test of the single values: each adds at most 1, so a NaN or +inf among them shows in the sum, and they are
+  // cleaned then.
+  add();
+  if (!(sum <= 8.5f * N)) {
+#pragma unroll
+    for (int j = 0; j < 8 * N; ++j) v[j] = clean_logit<T>(v[j]);
+    top = clean_logit<T>(top);
+    add();
+  }
+}
+
+// grid: (chunks / warps per CTA, sequences, row_step). A warp takes one chunk of every row_step-th row of its
+// sequence, so that its offsets and temperature are one round of loads, whatever the sequences' lengths. A
+// chunk starts on a 16-byte boundary: chunk c of a row whose first value lies `head` values past one covers the
+// columns [n c - head, n (c + 1) - head), n = chunk_cols. 512 or 1024 columns at a time, the next ones requested under the
+// current ones'; each lane keeps a maximum and a sum of its own, joined by shuffles at the end.
+template <typename T>
+__global__ void __launch_bounds__(kVfyThreads) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31;
+  const int chunk = static_cast<int>(blockIdx.x) * kVfyWarps + static_cast<int>(threadIdx.x >> 5);
+  if (chunk >= a.n_chunks) return;
+  for (int64_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    const int64_t lo = clamp_offset(__ldg(a.cu + b), a.n_drafts);
+    const int64_t hi = max(lo, clamp_offset(__ldg(a.cu + b + 1), a.n_drafts));
+    const SeqTemp st = seq_temp(a, b);
+    const float k = kLog2e / st.t;
+    for (int64_t row = lo + b + blockIdx.z; row <= hi + b; row += a.row_step) {
+      const T* z = static_cast<const T*>(a.logits) + row * a.ld_logits;
+      const int head = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+      const int64_t first = static_cast<int64_t>(chunk) * a.chunk_cols - head;  // column of the chunk's first vector
+      const int64_t end = min(a.vocab, first + a.chunk_cols);
+      RowStats r{-kFltMax, 0.0f, 0xFFFFFFFFu};
+      int c = static_cast<int>(first) + lane * 8;
+      const T* zp = z + c;
+      const int vocab = static_cast<int>(a.vocab);
+      auto load = [&](int ahead, Vec8<T>& v) {
+        const int at = c + ahead;
+        if (at >= 0 && at + 8 <= vocab)
+          v.load(zp + ahead);
+        else
+          v.load_some(zp + ahead, 1, -at, vocab - at, Vec8<T>::kNegInf);
+      };
+      constexpr int kVec = sizeof(T) == 4 ? 2 : 4;  // 64 bytes in flight per lane
+      Vec8<T> nxt[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) load(256 * i, nxt[i]);
+#pragma unroll 1
+      for (int n = static_cast<int>(end - first); n > 0; n -= 256 * kVec) {
+        Vec8<T> cur[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) cur[i] = nxt[i];
+        if (n > 256 * kVec) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) load(256 * (kVec + i), nxt[i]);
+        }
+        add_vectors<T, kVec>(r, cur, k, st.greedy, static_cast<uint32_t>(c));
+        c += 256 * kVec;
+        zp += 256 * kVec;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        RowStats x;
+        x.m = __shfl_xor_sync(0xffffffffu, r.m, o);
+        x.s = __shfl_xor_sync(0xffffffffu, r.s, o);
+        x.idx = __shfl_xor_sync(0xffffffffu, r.idx, o);
+        join_stats(r, x, k);
+      }
+      if (lane == 0) a.partials[row * a.n_chunks + chunk] = make_float4(r.m, r.s, __uint_as_float(r.idx), 0.0f);
+    }
+  }
+}
+
+// Statistics of one whole row, the same in every lane.
 __device__ __forceinline__ RowStats merge_row(const VerifyArgs& a, int64_t row, float t, int lane) {
   const float4* p = a.partials + row * a.n_chunks;
-  RowStats r{-INFINITY, 0.0, 0xFFFFFFFFu};
-  for (int c = lane; c < a.n_chunks; c += 32) r.m = fmaxf(r.m, p[c].x);
+  const float k = kLog2e / t;
+  RowStats r{-kFltMax, 0.0f, 0xFFFFFFFFu};
+#pragma unroll 1
+  for (int c0 = lane; c0 < a.n_chunks; c0 += 128) {
+    float4 v[4];  // four loads in flight
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
-  if (r.m == -INFINITY) return r;
-  for (int c = lane; c < a.n_chunks; c += 32) {
-    const float4 v = p[c];
-    if (v.x == -INFINITY) continue;
-    r.s += static_cast<double>(v.y) * exp((static_cast<double>(v.x) - r.m) / t);
-    if (v.x == r.m) r.idx = min(r.idx, __float_as_uint(v.z));
+    for (int i = 0; i < 4; ++i)
+      v[i] = c0 + 32 * i < a.n_chunks ? ld_dep_v4(p + c0 + 32 * i) : make_float4(-kFltMax, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) join_stats(r, RowStats{v[i].x, v[i].y, __float_as_uint(v[i].z)}, k);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
-  r.idx = __reduce_min_sync(0xffffffffu, r.idx);
+  for (int o = 16; o > 0; o >>= 1) {
+    RowStats x;
+    x.m = __shfl_xor_sync(0xffffffffu, r.m, o);
+    x.s = __shfl_xor_sync(0xffffffffu, r.s, o);
+    x.idx = __shfl_xor_sync(0xffffffffu, r.idx, o);
+    join_stats(r, x, k);
+  }
   return r;
 }
 
@@ -218,6 +357,22 @@ __device__ __forceinline__ double ld_cluster_f64(const double* local, uint32_t r
   return v;
 }
 
+// How many drafts of a sequence passed, and the maximum and sum of the row that its next token comes from.
+struct __align__(16) Decision {
+  int64_t acc;
+  float m, s;
+};
+
+// The same variable of CTA `rank` of the cluster.
+__device__ __forceinline__ Decision ld_cluster_decision(const Decision* local, uint32_t rank) {
+  Decision d;
+  asm volatile("{\n\t.reg .b64 t;\n\tld.shared::cluster.v2.b64 {%0, t}, [%3];\n\tmov.b64 {%1, %2}, t;\n\t}"
+               : "=l"(d.acc), "=f"(d.m), "=f"(d.s)
+               : "r"(map_to_cta(smem_u32(local), rank))
+               : "memory");
+  return d;
+}
+
 // What the next token is drawn from.
 enum DrawMode : int { kDrawP = 0, kDrawWithout = 1, kDrawResidual = 2 };
 
@@ -225,39 +380,114 @@ struct DrawRow {
   const void* z;
   const void* q;
   double m;
-  double inv_t;
-  double inv_s;
-  int64_t without;  // kDrawWithout: the token taken out
+  double scale;  // 1024 log2(e) / T: exp((z - m) / T) = 2^((z - m) scale / 1024)
+  float floor;   // logits below have weight 0: m - 680 T, where exp is 4e-296
+  int without;  // kDrawWithout: the token taken out, else -1
   int mode;
 };
 
-// Weights of eight consecutive columns from c (those below `end`; others 0).
-template <typename T, typename Q>
-__device__ __forceinline__ void weights8(const VerifyArgs& a, const DrawRow& d, int64_t c, int64_t end,
-                                         double (&w)[8]) {
-  float z[8], q[8];
-  load8<T>(static_cast<const T*>(d.z) + c, a.logits_vec != 0, end - c, -INFINITY, z);
-  if (d.mode == kDrawResidual) load8<Q>(static_cast<const Q*>(d.q) + c, a.q_vec != 0, end - c, 0.0f, q);
+// Weight of one column of the drawn row from its logit and (kResidual) draft probability. `live` false: the
+// column has no weight and the value returned is some number. A residual of exactly 0 counts as live.
+template <typename T, typename Q, bool kResidual>
+__device__ __forceinline__ double draw_weight(const DrawRow& d, const double* table, float z, float q, bool& live) {
+  constexpr float kCap = sizeof(T) == 4 ? kFltMax : 3.38953139e38f;  // as clean_logit
+  double w = exp2_scaled(widen<T>(fminf(z, kCap)) - d.m, d.scale, table);
+  live = z >= d.floor;  // false for NaN
+  if (kResidual) {
+    w -= widen_prob<Q>(q);
+    live = live && __double2hiint(w) >= 0;
+  }
+  return w;
+}
+
+// Eight columns of the drawn row as they are read: `n` of them from zp and qp on with that step are there (others
+// count as masked). vec: whole vectors may be loaded (step 1).
+template <typename T, typename Q, bool kResidual>
+struct DrawCols {
+  Vec8<T> z;
+  Vec8<Q> q;
+  __device__ __forceinline__ void load(const T* zp, const Q* qp, int step, int n, bool vec) {
+    if (vec && n >= 8) {
+      z.load(zp);
+      if (kResidual) q.load(qp);
+    } else {
+      z.load_some(zp, step, 0, n, Vec8<T>::kNegInf);
+      if (kResidual) q.load_some(qp, step, 0, n, 0);
+    }
+  }
+};
+
+// kDrawWithout: masks the token that is taken out in the columns c + j * step, if it is among them.
+template <typename T>
+__device__ __forceinline__ void mask_without(const DrawRow& d, Vec8<T>& z, int c, int step) {
+  if (d.without >= c && d.without < c + 8 * step) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float zc = clean_logit(z[j]);
-    double p = zc == -INFINITY ? 0.0 : exp((static_cast<double>(zc) - d.m) * d.inv_t) * d.inv_s;
-    if (d.mode == kDrawResidual) p = fmax(p - static_cast<double>(fmaxf(q[j], 0.0f)), 0.0);
-    if (d.mode == kDrawWithout && c + j == d.without) p = 0.0;
-    w[j] = p;
+    for (int j = 0; j < 8; ++j)
+      if (c + j * step == d.without) z.mask(j);
   }
 }
 
+// Sum of this lane's weights over the columns [lo, hi) of its warp; the sums over each group of group_cols columns
+// go to s_lane[group][thread].
+template <typename T, typename Q, bool kResidual>
+__device__ __forceinline__ double sum_columns(const VerifyArgs& a, const DrawRow& d, const double* table, int lo, int hi,
+                                              int group_cols, double (*s_lane)[kVfyThreads]) {
+  const int lane = threadIdx.x & 31;
+  const bool vec = a.logits_vec != 0 && (!kResidual || a.q_vec != 0);
+  // whole vectors, or coalesced single values (a sum does not care for the order)
+  const int step = vec ? 1 : 32;
+  int c = lo + (vec ? lane * 8 : lane);
+  const T* zp = static_cast<const T*>(d.z) + c;
+  const Q* qp = static_cast<const Q*>(d.q) + c;
+  DrawCols<T, Q, kResidual> nxt;
+  nxt.load(zp, qp, step, hi - c, vec);
+  double all = 0.0;
+  int g = 0;
+#pragma unroll 1
+  for (int g0 = lo; g0 < hi; g0 += group_cols, ++g) {
+    const int strips = (min(hi - g0, group_cols) + 255) >> 8;
+    double sum = 0.0, sum1 = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < strips; ++i) {
+      DrawCols<T, Q, kResidual> cur = nxt;
+      zp += 256;
+      qp += 256;
+      nxt.load(zp, qp, step, hi - c - 256, vec);  // behind the last column nothing is read
+      if (!kResidual) mask_without(d, cur.z, c, step);
+      c += 256;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        bool live;
+        const double w = draw_weight<T, Q, kResidual>(d, table, cur.z.at(j), kResidual ? cur.q.at(j) : 0.0f, live);
+        if (live) {
+          if (j & 1)
+            sum1 += w;
+          else
+            sum += w;
+        }
+      }
+    }
+    sum += sum1;
+    s_lane[g][threadIdx.x] = sum;
+    all += sum;
+  }
+  return all;
+}
+
 template <typename T, typename Q>
-__global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThreads) verify_sample_kernel(VerifyArgs a) {
-  __shared__ int s_pass[kVfyThreads];
-  __shared__ float s_logp[kVfyThreads];
+__global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __grid_constant__ VerifyArgs a) {
+  __shared__ int s_pass[kVfyWarps];
+  __shared__ double s_x[kVfyWarps];
+  __shared__ Decision s_decision;
   __shared__ double s_warp[kVfyWarps];
   __shared__ double s_total[2];  // read by the other CTAs of the cluster; one per exchange
-  __shared__ RowStats s_row;
+  __shared__ RowStats s_rows[kVfyWarps];
+  __shared__ double s_exp2[kExp2Entries];  // over the softmax denominator where weights are probabilities
+  __shared__ double s_lane[kVfyMaxGroups][kVfyThreads];  // a lane's sum over each of its warp's groups of columns
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = cluster_cta_rank();
-  const int64_t b = blockIdx.x / kVfyCluster;
+  const uint32_t rank = cluster_cta_rank(), ctas = cluster_cta_count();
+  const int64_t b = blockIdx.x / ctas;
+  for (int j = threadIdx.x; j < kExp2Entries; j += kVfyThreads) s_exp2[j] = a.exp2.coarse[j >> 5] * a.exp2.fine[j & 31];
   const int64_t c_lo = __ldg(a.cu + b), c_hi = __ldg(a.cu + b + 1);
   const int64_t lo = clamp_offset(c_lo, a.n_drafts);
   const int64_t hi = max(lo, clamp_offset(c_hi, a.n_drafts));
@@ -269,56 +499,65 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
   const SeqTemp st = seq_temp(a, b);
   const T* logits = static_cast<const T*>(a.logits);
 
-  // ---- how many drafts pass: kVfyWarps at a time, every CTA of the cluster for itself
-  int64_t acc = n;
-  for (int64_t i0 = 0; i0 < n && acc == n; i0 += kVfyWarps) {
-    const int64_t i = i0 + warp;
-    if (i < n) {
-      const RowStats r = merge_row(a, row0 + i, st.t, lane);
-      const int64_t d = __ldg(a.drafts + lo + i);
-      const bool valid = d >= 0 && d < a.vocab;
-      int pass = 0;
-      float logp = 0.0f;
-      if (valid && r.m > -INFINITY) {
-        const float z = clean_logit(to_f32<T>(logits[(row0 + i) * a.ld_logits + d]));
-        const double x = (static_cast<double>(z) - r.m) / st.t;
-        logp = static_cast<float>(x - log(r.s));
-        if (st.greedy) {
-          pass = static_cast<uint32_t>(d) == r.idx;
-        } else {
-          const double qd =
-              a.q == nullptr ? 1.0 : fmaxf(to_f32<Q>(static_cast<const Q*>(a.q)[(lo + i) * a.ld_q + d]), 0.0f);
-          pass = static_cast<double>(__ldg(a.uniforms + lo + i)) * qd < exp(x) / r.s;
+  // ---- how many drafts pass: the cluster's first CTA decides, kVfyWarps rows at a time, and hands the result to
+  // the others through its shared memory. What does not depend on the statistics is loaded before the wait for
+  // them. Row n has no draft to pass.
+  if (rank == 0) {
+    int64_t acc = -1;
+#pragma unroll 1
+    for (int64_t i0 = 0; acc < 0; i0 += kVfyWarps) {
+      const int64_t i = i0 + warp;
+      if (i <= n) {
+        int64_t d = -1;
+        bool valid = false;
+        float z = -INFINITY, qd = 1.0f, u = 0.0f;
+        if (i < n) {
+          d = __ldg(a.drafts + lo + i);
+          u = __ldg(a.uniforms + lo + i);
+          valid = d >= 0 && d < a.vocab;
+          if (valid) {
+            z = clean_logit<T>(to_f32<T>(logits[(row0 + i) * a.ld_logits + d]));
+            if (a.q != nullptr) qd = fmaxf(to_f32<Q>(static_cast<const Q*>(a.q)[(lo + i) * a.ld_q + d]), 0.0f);
+          }
+        }
+        grid_dep_wait();
+        const RowStats r = merge_row(a, row0 + i, st.t, lane);
+        if (lane == 0) {
+          const double x = (static_cast<double>(z) - r.m) / st.t;
+          int pass = 0;
+          if (valid && r.s > 0.0f)
+            pass = st.greedy ? static_cast<uint32_t>(d) == r.idx : static_cast<double>(u) * qd * r.s < exp(x);
+          s_pass[warp] = valid || i == n ? pass : -1;
+          s_x[warp] = x;
+          s_rows[warp] = r;
         }
       }
-      if (lane == 0) {
-        s_pass[warp] = valid ? pass : -1;
-        s_logp[warp] = logp;
+      __syncthreads();
+      for (int w = 0; w < kVfyWarps && i0 + w <= n; ++w)
+        if (s_pass[w] != 1) {
+          acc = i0 + w;
+          break;
+        }
+      const int64_t upto = acc < 0 ? i0 + kVfyWarps : acc;
+      if (threadIdx.x < kVfyWarps && i0 + threadIdx.x < upto) {
+        a.tokens[row0 + i0 + threadIdx.x] = __ldg(a.drafts + lo + i0 + threadIdx.x);
+        a.log_probs[row0 + i0 + threadIdx.x] =
+            static_cast<float>(s_x[threadIdx.x] - log(static_cast<double>(s_rows[threadIdx.x].s)));
       }
-    }
-    __syncthreads();
-    int64_t stop = -1;
-    for (int w = 0; w < kVfyWarps && i0 + w < n; ++w)
-      if (s_pass[w] != 1) {
-        stop = w;
-        break;
+      if (acc >= 0 && threadIdx.x == 0) {
+        const RowStats r = s_rows[acc - i0];
+        s_decision = {acc, r.m, r.s};
+        if (s_pass[acc - i0] < 0 && a.status != nullptr) atomicOr(a.status, kStatusBadTarget);
+        a.accepted[b] = acc;
+        if (r.s == 0.0f || st.greedy) {  // nothing to draw
+          a.tokens[row0 + acc] = r.s == 0.0f ? -1 : static_cast<int64_t>(r.idx);
+          a.log_probs[row0 + acc] = r.s == 0.0f ? -INFINITY : static_cast<float>(-log(static_cast<double>(r.s)));
+        }
       }
-    if (stop >= 0) acc = i0 + stop;
-    if (rank == 0 && threadIdx.x < kVfyWarps && i0 + threadIdx.x < acc) {
-      a.tokens[row0 + i0 + threadIdx.x] = __ldg(a.drafts + lo + i0 + threadIdx.x);
-      a.log_probs[row0 + i0 + threadIdx.x] = s_logp[threadIdx.x];
+      __syncthreads();
     }
-    if (first_thread && stop >= 0 && s_pass[stop] < 0 && a.status != nullptr) atomicOr(a.status, kStatusBadTarget);
-    __syncthreads();
-  }
-  const int64_t row = row0 + acc;
-  if (warp == 0) {
-    const RowStats r = merge_row(a, row, st.t, lane);
-    if (lane == 0) s_row = r;
-  }
-  if (rank == 0) {
     const int64_t last = b == a.batch - 1 ? a.n_drafts + a.batch - 1 : row0 + n;
-    for (int64_t i = row + 1 + threadIdx.x; i <= last; i += kVfyThreads) {
+    for (int64_t i = row0 + acc + 1 + threadIdx.x; i <= last; i += kVfyThreads) {
       a.tokens[i] = -1;
       a.log_probs[i] = 0.0f;
     }
@@ -328,16 +567,13 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
         a.log_probs[i] = 0.0f;
       }
     }
-    if (threadIdx.x == 0) a.accepted[b] = acc;
   }
-  __syncthreads();
-  const RowStats rs = s_row;
-  // uniform over the cluster: no CTA of it reaches the exchanges below
-  if (rs.m == -INFINITY || st.greedy) {
-    if (first_thread) {
-      a.tokens[row] = rs.m == -INFINITY ? -1 : static_cast<int64_t>(rs.idx);
-      a.log_probs[row] = rs.m == -INFINITY ? -INFINITY : static_cast<float>(-log(rs.s));
-    }
+  cluster_sync_all();
+  const Decision decision = ld_cluster_decision(&s_decision, 0);
+  const int64_t acc = decision.acc, row = row0 + acc;
+  const RowStats rs = {decision.m, decision.s, 0};
+  if (rs.s == 0.0f || st.greedy) {
+    cluster_sync_all();  // the first CTA stays until all have read its decision
     return;
   }
 
@@ -346,25 +582,23 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
   d.z = logits + row * a.ld_logits;
   d.q = a.q == nullptr ? nullptr : static_cast<const Q*>(a.q) + (lo + acc) * a.ld_q;
   d.m = rs.m;
-  d.inv_t = 1.0 / st.t;
-  d.inv_s = 1.0;
+  d.floor = rs.m - 680.0f * st.t;
+  d.scale = kExp2Entries * 1.4426950408889634074 / st.t;
   d.without = -1;
   d.mode = kDrawP;
-  // columns of this CTA, and of each of its warps, in order
-  const int64_t per_warp = (((a.vocab + kVfyCluster * kVfyWarps - 1) / (kVfyCluster * kVfyWarps)) + 255) / 256 * 256;
-  const int64_t w_lo = min(a.vocab, (static_cast<int64_t>(rank) * kVfyWarps + warp) * per_warp);
-  const int64_t w_hi = min(a.vocab, w_lo + per_warp);
+  // columns of this CTA, and of each of its warps, in order, in groups of strip_step strips of 256
+  const int group_cols = 256 * a.strip_step;
+  const int warps = static_cast<int>(ctas) * kVfyWarps;
+  const int64_t per_warp = ((a.vocab + warps - 1) / warps + group_cols - 1) / group_cols * group_cols;
+  const int w_lo = static_cast<int>(min(a.vocab, (static_cast<int64_t>(rank) * kVfyWarps + warp) * per_warp));
+  const int w_hi = static_cast<int>(min(a.vocab, w_lo + per_warp));
   int exchange = 0;
-  double total = 0.0, before = 0.0, mine = 0.0;
+  double total = 0.0, before = 0.0, mine = 0.0, theirs = 0.0;
   // This warp's sum of weights (mine), the sum of all columns before this CTA's (before) and of all
-  // columns (total).
+  // columns (total); the lanes' sums of each group stay in s_lane.
   auto sum_weights = [&]() {
-    mine = 0.0;
-    for (int64_t c = w_lo + lane * 8; c < w_hi; c += 256) {
-      double w[8];
-      weights8<T, Q>(a, d, c, w_hi, w);
-      mine += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-    }
+    mine = d.mode == kDrawResidual ? sum_columns<T, Q, true>(a, d, s_exp2, w_lo, w_hi, group_cols, s_lane)
+                                   : sum_columns<T, Q, false>(a, d, s_exp2, w_lo, w_hi, group_cols, s_lane);
     mine = warp_sum(mine);
     __syncthreads();
     if (lane == 0) s_warp[warp] = mine;
@@ -375,47 +609,51 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
       s_total[exchange] = t;
     }
     cluster_sync_all();
+    // lane k reads CTA k's sum, so that the reads are in flight together
+    theirs = static_cast<uint32_t>(lane) < ctas ? ld_cluster_f64(&s_total[exchange], lane) : 0.0;
     total = before = 0.0;
-    for (uint32_t k = 0; k < kVfyCluster; ++k) {
-      const double t = ld_cluster_f64(&s_total[exchange], k);
+    for (uint32_t k = 0; k < ctas; ++k) {
+      const double t = __shfl_sync(0xffffffffu, theirs, static_cast<int>(k));
       if (k < rank) before += t;
       total += t;
     }
     exchange ^= 1;
   };
-  if (acc < n && a.q != nullptr) {
-    sum_weights();  // the softmax denominator in 64 bits
-    d.inv_s = 1.0 / total;
-    d.mode = kDrawResidual;
-    sum_weights();
-    if (!(total > 0.0)) {
-      d.mode = kDrawP;
-      sum_weights();
-    }
-  } else {
-    if (acc < n) {
+  // One copy of the pass, so that its code stays in the instruction cache: with draft probabilities first the
+  // softmax denominator in 64 bits, then the weights, and p when nothing is left of those.
+  bool denominator = false;
+  if (acc < n) {
+    denominator = a.q != nullptr;
+    if (!denominator) {
       d.mode = kDrawWithout;
-      d.without = __ldg(a.drafts + lo + acc);
+      const int64_t t = __ldg(a.drafts + lo + acc);
+      d.without = t >= 0 && t < a.vocab ? static_cast<int>(t) : -1;
     }
+  }
+#pragma unroll 1
+  for (;;) {
     sum_weights();
-    if (!(total > 0.0)) {
+    if (denominator) {
+      denominator = false;
+      // every CTA has passed the exchange, so this one's warps are done with the table
+      const double inv = 1.0 / total;
+      for (int j = threadIdx.x; j < kExp2Entries; j += kVfyThreads) s_exp2[j] *= inv;
+      __syncthreads();
+      d.mode = kDrawResidual;
+    } else if (total > 0.0 || d.mode == kDrawP) {
+      break;
+    } else {
       d.mode = kDrawP;
-      sum_weights();
+      d.without = -1;
     }
   }
   // x = r * total falls to the last warp with any weight whose columns start at or before x (so exactly
-  // one takes it, whatever rounding does at the ends); that warp walks its columns again.
+  // one takes it, whatever rounding does at the ends).
   const float rf = __ldg(a.final_uniforms + b);
   const double x = (rf >= 0.0f ? fmin(static_cast<double>(rf), 1.0) : 0.0) * total;
-  double after = before;  // where the next CTA's columns start
-  bool later = false;     // a later CTA has weight
-  for (uint32_t k = rank; k < kVfyCluster; ++k) {
-    const double t = ld_cluster_f64(&s_total[exchange ^ 1], k);
-    if (k == rank)
-      after += t;
-    else
-      later = later || t > 0.0;
-  }
+  // where the next CTA's columns start, and whether a later CTA has weight
+  const double after = before + __shfl_sync(0xffffffffu, theirs, static_cast<int>(rank));
+  const bool later = __any_sync(0xffffffffu, static_cast<uint32_t>(lane) > rank && theirs > 0.0);
   double start = before, next = later ? after : INFINITY;
   {
     double run = before;
@@ -432,24 +670,58 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
   }
   const bool takes = mine > 0.0 && start <= x && x < next;
   if (takes) {
-    double run = start;
-    int64_t token = -1, last_live = -1;
-    double zx = 0.0;
-    for (int64_t c0 = w_lo; c0 < w_hi && token < 0; c0 += 256) {
-      const int64_t c = c0 + lane * 8;
-      double w[8];
-      if (c < w_hi) {
-        weights8<T, Q>(a, d, c, w_hi, w);
-      } else {
+    // The last group with any weight that starts at or before x, from the kept sums; then its strips.
+    // lane g: the sum of group g, and of those before it
+    double group_sum = 0.0;
+    const int groups = (w_hi - w_lo + group_cols - 1) / group_cols;
+#pragma unroll 4
+    for (int g = 0; g < groups; ++g) {
+      const double sum = warp_sum(s_lane[g][threadIdx.x]);
+      if (lane == g) group_sum = sum;
+    }
+    double upto = group_sum;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = 0.0;
+    for (int o = 1; o < kVfyMaxGroups; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    double run = fmax(start + (upto - group_sum), start);
+    const uint32_t starts = __ballot_sync(0xffffffffu, group_sum > 0.0 && run <= x);
+    const int g = starts != 0 ? 31 - __clz(starts) : 0;  // the first live group starts at `start`, so there is one
+    run = __shfl_sync(0xffffffffu, run, g);
+    const int at = w_lo + g * group_cols;
+    const int g1 = min(w_hi, at + group_cols);
+    int token = -1, last_live = -1;
+#pragma unroll 1
+    for (int c0 = at; c0 < g1 && token < 0; c0 += 256) {
+      const int c = c0 + lane * 8;
+      const T* zp = static_cast<const T*>(d.z) + c;
+      const Q* qp = static_cast<const Q*>(d.q) + c;
+      double w[8];
+      bool is_live[8];
+      if (d.mode == kDrawResidual) {
+        DrawCols<T, Q, true> cols;
+        cols.load(zp, qp, 1, g1 - c, a.logits_vec != 0 && a.q_vec != 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          w[j] = draw_weight<T, Q, true>(d, s_exp2, cols.z.at(j), cols.q.at(j), is_live[j]);
+          is_live[j] = is_live[j] && w[j] > 0.0;
+        }
+      } else {
+        DrawCols<T, Q, false> cols;
+        cols.load(zp, qp, 1, g1 - c, a.logits_vec != 0);
+        mask_without(d, cols.z, c, 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = draw_weight<T, Q, false>(d, s_exp2, cols.z.at(j), 0.0f, is_live[j]);
       }
       double sum = 0.0;
       int live = -1;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        sum += w[j];
-        if (w[j] > 0.0) live = j;
+        if (is_live[j]) {
+          sum += w[j];
+          live = j;
+        }
       }
       double incl = sum;
 #pragma unroll
@@ -461,8 +733,10 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
       int hit = -1;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        cur += w[j];
-        if (hit < 0 && w[j] > 0.0 && cur > x) hit = j;
+        if (is_live[j]) {
+          cur += w[j];
+          if (hit < 0 && cur > x) hit = j;
+        }
       }
       const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0);
       const uint32_t lives = __ballot_sync(0xffffffffu, live >= 0);
@@ -475,31 +749,67 @@ __global__ void __cluster_dims__(kVfyCluster, 1, 1) __launch_bounds__(kVfyThread
       }
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (token < 0) token = last_live;
+    if (token < 0) token = last_live;  // what rounding leaves past the end
     if (lane == 0) {
-      zx = (static_cast<double>(clean_logit(to_f32<T>(static_cast<const T*>(d.z)[token]))) - d.m) * d.inv_t;
+      const double z = clean_logit<T>(to_f32<T>(static_cast<const T*>(d.z)[token]));
       a.tokens[row] = token;
-      a.log_probs[row] = static_cast<float>(zx - log(rs.s));
+      a.log_probs[row] = static_cast<float>((z - rs.m) / st.t - log(static_cast<double>(rs.s)));
     }
   }
   cluster_sync_all();  // no CTA leaves while another may still read its sums
 }
 
+// CTAs per sequence: as many as keep 8 clusters' worth of SMs busy with few sequences (one sequence of V = 32000:
+// 8), fewer when the batch fills the GPU anyway, since each CTA of a cluster repeats the decision.
+inline int verify_cluster(int64_t batch, int64_t vocab, int sms) {
+  int ctas = kVfyMaxCluster;
+  while (ctas > 1 && (batch * ctas > 4 * sms || vocab <= 256 * kVfyWarps * (ctas / 2))) ctas /= 2;
+  return ctas;
+}
+
 template <typename T, typename Q>
-static int launch_verify(const VerifyArgs& a, cudaStream_t stream) {
+static int launch_verify(VerifyArgs& a, cudaStream_t stream) {
+  int sms = 0;
+  int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int ctas = verify_cluster(a.batch, a.vocab, sms);
+  FRX_REQUIRE(a.batch * ctas < (1ll << 31), FRX_ERR_INVALID_ARG, "frx_verify_drafts: too many sequences (%lld)",
+              (long long)a.batch);
+  // a warp's columns in at most kVfyMaxGroups groups
+  const int64_t strips = (a.vocab + 256ll * ctas * kVfyWarps - 1) / (256ll * ctas * kVfyWarps);
+  a.strip_step = static_cast<int>((strips + kVfyMaxGroups - 1) / kVfyMaxGroups);
+  // Longer chunks spare a warp's set-up and its joins, as long as they leave the GPU 32 warps per SM.
+  a.chunk_cols = kVfyChunk;
   const int64_t rows = a.n_drafts + a.batch;
-  const int64_t blocks = (rows * a.n_chunks + kVfyWarps - 1) / kVfyWarps;
-  FRX_REQUIRE(blocks < (1ll << 31) && a.batch * kVfyCluster < (1ll << 31), FRX_ERR_INVALID_ARG,
-              "frx_verify_drafts: problem too large (%lld rows, %lld columns)", (long long)rows, (long long)a.vocab);
-  verify_stats_kernel<T><<<static_cast<unsigned>(blocks), kVfyThreads, 0, stream>>>(a);
+  while (a.chunk_cols < 16 * kVfyChunk && rows * ((a.vocab + 2 * a.chunk_cols - 1) / (2 * a.chunk_cols)) >= 32ll * sms)
+    a.chunk_cols *= 2;
+  a.n_chunks = static_cast<int>((a.vocab + 7 + a.chunk_cols - 1) / a.chunk_cols);
+  const int64_t mean_rows = (a.n_drafts + 2 * a.batch - 1) / a.batch;
+  a.row_step = static_cast<int>(mean_rows < 64 ? mean_rows : 64);
+  const dim3 grid(static_cast<unsigned>((a.n_chunks + kVfyWarps - 1) / kVfyWarps),
+                  static_cast<unsigned>(a.batch < 65535 ? a.batch : 65535), static_cast<unsigned>(a.row_step));
+  verify_stats_kernel<T><<<grid, kVfyThreads, 0, stream>>>(a);
   FRX_CUDA_CHECK(cudaGetLastError());
-  verify_sample_kernel<T, Q><<<static_cast<unsigned>(a.batch * kVfyCluster), kVfyThreads, 0, stream>>>(a);
-  FRX_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch * ctas), 1, 1);
+  cfg.blockDim = dim3(kVfyThreads, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  FRX_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_sample_kernel<T, Q>, static_cast<const VerifyArgs>(a)));
   return FRX_OK;
 }
 
 template <typename T>
-static int launch_verify_q(const VerifyArgs& a, int q_dtype, cudaStream_t stream) {
+static int launch_verify_q(VerifyArgs& a, int q_dtype, cudaStream_t stream) {
   if (q_dtype == FRX_DTYPE_BF16) return launch_verify<T, __nv_bfloat16>(a, stream);
   if (q_dtype == FRX_DTYPE_F16) return launch_verify<T, __half>(a, stream);
   return launch_verify<T, float>(a, stream);
@@ -514,7 +824,7 @@ extern "C" int frx_verify_drafts(const void* logits, int dtype, int64_t ld_logit
                                  int64_t vocab, float* workspace, int64_t workspace_floats, int64_t* accepted,
                                  int64_t* tokens, float* log_probs, int* status, void* stream) {
   using namespace frx;
-  FRX_REQUIRE(batch >= 0 && n_drafts >= 0 && vocab >= 1 && vocab < (1ll << 31) && batch < (1ll << 31) &&
+  FRX_REQUIRE(batch >= 0 && n_drafts >= 0 && vocab >= 1 && vocab < (1ll << 30) && batch < (1ll << 31) &&
                   n_drafts < (1ll << 31) && ld_logits >= vocab,
               FRX_ERR_INVALID_ARG, "frx_verify_drafts: bad sizes batch=%lld n_drafts=%lld vocab=%lld ld_logits=%lld",
               (long long)batch, (long long)n_drafts, (long long)vocab, (long long)ld_logits);
@@ -535,7 +845,7 @@ extern "C" int frx_verify_drafts(const void* logits, int dtype, int64_t ld_logit
                   (n_drafts == 0 || (drafts != nullptr && uniforms != nullptr)),
               FRX_ERR_INVALID_ARG, "frx_verify_drafts: null pointer");
   const int64_t rows = n_drafts + batch;
-  const int64_t n_chunks = (vocab + kVfyChunk - 1) / kVfyChunk;
+  const int64_t n_chunks = (vocab + 7 + kVfyChunk - 1) / kVfyChunk;
   FRX_REQUIRE(aligned16(workspace) && workspace_floats >= 4 * rows * n_chunks, FRX_ERR_INVALID_ARG,
               "frx_verify_drafts: workspace must be 16-byte aligned with 4 * %lld * %lld floats (got %lld)",
               (long long)rows, (long long)n_chunks, (long long)workspace_floats);
@@ -552,7 +862,9 @@ extern "C" int frx_verify_drafts(const void* logits, int dtype, int64_t ld_logit
   FRX_CHECK_RANGE(accepted, batch * 8, "frx_verify_drafts: accepted");
   FRX_CHECK_RANGE(tokens, rows * 8, "frx_verify_drafts: tokens");
   FRX_CHECK_RANGE(log_probs, rows * 4, "frx_verify_drafts: log_probs");
+  static const Exp2Table exp2 = make_exp2_table();
   VerifyArgs a = {};
+  a.exp2 = exp2;
   a.logits = logits;
   a.ld_logits = ld_logits;
   a.logits_vec = aligned16(logits) && (ld_logits * esz) % 16 == 0;
@@ -568,7 +880,6 @@ extern "C" int frx_verify_drafts(const void* logits, int dtype, int64_t ld_logit
   a.batch = batch;
   a.n_drafts = n_drafts;
   a.vocab = vocab;
-  a.n_chunks = static_cast<int>(n_chunks);
   a.partials = reinterpret_cast<float4*>(workspace);
   a.accepted = accepted;
   a.tokens = tokens;

@@ -43,9 +43,11 @@ def __getattr__(name):
     if name in _INT8_HEAD_NAMES:
         from fast_reduction import int8_head
 
-        return getattr(int8_head, name)
+        value = globals()[name] = getattr(int8_head, name)  # found directly from now on
+        return value
     if name == "verify_drafts":
         from fast_reduction import draft_verify
 
-        return draft_verify.verify_drafts
+        value = globals()[name] = draft_verify.verify_drafts
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -57,7 +57,8 @@ def verify_drafts(
     the rejected token taken out; from p when nothing is left), or from the last row's p: the first j whose
     running sum of weights passes final_uniforms[b] times their total.
 
-    target_logits   [N + B, V] bf16 / fp16 / fp32; NaN counts as -inf, +inf as the largest float
+    target_logits   [N + B, V] bf16 / fp16 / fp32; NaN counts as -inf, +inf as the largest finite
+                    value (of fp32 for fp32 logits, of bf16 for 16-bit ones)
     draft_tokens    [N] int32 / int64; an id outside [0, V) is rejected and sets FRX_STATUS_BAD_TARGET
     cu_drafts       [B + 1] int32 / int64 on the GPU, from 0, non-decreasing; its last entry may be below N (a
                     padded batch: rows behind the last sequence's are not read)
@@ -88,8 +89,7 @@ def verify_drafts(
     accepted = torch.empty(batch, device=dev, dtype=torch.int64)
     tokens = torch.empty(rows, device=dev, dtype=torch.int64)
     log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
-    workspace = torch.empty(4 * rows * ((vocab + nat.FRX_VERIFY_CHUNK - 1) // nat.FRX_VERIFY_CHUNK), device=dev,
-                            dtype=torch.float32)
+    workspace = torch.empty(4 * rows * ((vocab + 6) // nat.FRX_VERIFY_CHUNK + 1), device=dev, dtype=torch.float32)
     ops.verify_drafts(logits, drafts, cu, uniforms.contiguous(), final_uniforms.contiguous(), draft_probs, temps,
                       float(temperature), workspace, accepted, tokens, log_probs)
     return accepted, tokens, log_probs

@@ -173,9 +173,14 @@ def int8_ce_entropy(
     dev = x.device
     ce, ent, logp = torch.empty(3, B, device=dev, dtype=torch.float32).unbind(0)
     if B:
-        tiles = ops.n_vocab_tiles(w.shape[0])
-        chunk = gk._launch_rows(chunk, B, tiles)
-        workspace = torch.empty(ops.i8_workspace_bytes(x) + 16 * tiles * chunk, device=dev, dtype=torch.uint8)
+        V = w.shape[0]
+        if B <= nat.FRX_I8_FEW_ROWS:
+            partials = (V + 127) // 128 * B
+        else:
+            tiles = ops.n_vocab_tiles(V)
+            chunk = gk._launch_rows(chunk, B, tiles)
+            partials = tiles * chunk
+        workspace = torch.empty(ops.i8_workspace_bytes(x) + 16 * partials, device=dev, dtype=torch.uint8)
         ops.i8_ce_entropy(x, x_scale, w, w_scale, target, ce, ent, logp, workspace, launch_rows=chunk,
                           ignore_index=ignore_index, bias=bias)
     if hidden.dim() == 2:

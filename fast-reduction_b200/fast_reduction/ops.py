@@ -479,13 +479,33 @@ _I8_X_DTYPES = {**_OUT_DTYPES, torch.int8: nat.FRX_DTYPE_I8}
 def _call(name: str, entry: str, dev: torch.device, *args) -> None:
     """One libfrx call on the tensors' device, whatever the current one is, with its status word and stream last."""
     fn = getattr(nat.load(), entry)
-    if dev.index == torch.cuda.current_device():
-        rc = _launch(name, dev, lambda: fn(*args, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
-    else:
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            rc = _launch(name, dev, lambda: fn(*args, nat.status_word(dev).data_ptr(), nat.stream_of(dev)))
+            return _call(name, entry, dev, *args)
+    status, stream = nat.status_word(dev).data_ptr(), nat.stream_of(dev)
+    if _observer is None and not _NVTX:
+        rc = fn(*args, status, stream)
+    else:
+        rc = _launch(name, dev, lambda: fn(*args, status, stream))
     if rc:
         nat.check(rc, entry)
+
+
+def _one_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
+    """_require_cuda, with its loop left to the case that it refuses."""
+    dev = first.device
+    if dev.type == "cuda":
+        for t in rest:
+            if t is not None and t.device != dev:
+                break
+        else:
+            return dev
+    return _require_cuda(first, *rest)
+
+
+def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
+    return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 
 
 def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
@@ -520,23 +540,22 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias):
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
     if x.stride(1) != 1 or weight.stride(1) != 1:
         raise ValueError("x and weight must have unit column stride")
-    if weight_scale.dtype != torch.float32 or weight_scale.shape != (cols,) or not weight_scale.is_contiguous():
+    if not _is_vector(weight_scale, torch.float32, cols):
         raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
                          f"{tuple(weight_scale.shape)}")
     if x_scale is None:
         if x.dtype == torch.int8:
             raise ValueError("int8 tokens need their scales (hidden_scale)")
-    elif x.dtype != torch.int8 or x_scale.dtype != torch.float32 or x_scale.shape != (rows,) \
-            or not x_scale.is_contiguous():
+    elif x.dtype != torch.int8 or not _is_vector(x_scale, torch.float32, rows):
         raise ValueError(f"hidden_scale goes with int8 tokens, contiguous float32 [{rows}]")
     bptr, bdt = None, 0
     if bias is not None:
         bdt = _OUT_DTYPES.get(bias.dtype)
-        if bdt is None or bias.shape != (cols,) or not bias.is_contiguous():
+        if bdt is None or not _is_vector(bias, bias.dtype, cols):
             raise ValueError(f"bias must be a contiguous bfloat16, float16 or float32 [{cols}], got {bias.dtype} "
                              f"{tuple(bias.shape)}")
         bptr = bias.data_ptr()
-    dev = _require_cuda(x, x_scale, weight, weight_scale, bias)
+    dev = _one_device(x, x_scale, weight, weight_scale, bias)
     return dev, rows, cols, k, (x.data_ptr(), xdt, max(x.stride(0), k), None if x_scale is None else x_scale.data_ptr(),
                                 weight.data_ptr(), max(weight.stride(0), k), weight_scale.data_ptr(), bptr, bdt)
 
@@ -576,39 +595,38 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
     """accepted, tokens, log_probs <- the outcome of drafted tokens against target logits (frx_verify_drafts)."""
     n, batch = drafts.numel(), cu_drafts.numel() - 1
     dt = _LOGITS_DTYPES.get(logits.dtype)
-    if dt is None or logits.dim() != 2 or logits.shape[0] != n + batch or logits.stride(1) != 1:
+    rows, vocab = logits.shape
+    ldl, unit = logits.stride()
+    if dt is None or rows != n + batch or unit != 1:
         raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V] with unit column stride, got "
                          f"{logits.dtype} {tuple(logits.shape)} stride {logits.stride()}")
-    vocab = logits.shape[1]
     qptr, qdt, ldq = None, 0, 0
     if draft_probs is not None:
         qdt = _LOGITS_DTYPES.get(draft_probs.dtype)
-        if qdt is None or draft_probs.shape != (n, vocab) or draft_probs.stride(1) != 1:
+        ldq, unit = draft_probs.stride()
+        if qdt is None or draft_probs.shape != (n, vocab) or unit != 1:
             raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}] with unit column stride, "
                              f"got {draft_probs.dtype} {tuple(draft_probs.shape)} stride {draft_probs.stride()}")
-        qptr, ldq = draft_probs.data_ptr(), max(draft_probs.stride(0), vocab)
-    if drafts.dtype != torch.int64 or not drafts.is_contiguous():
-        raise ValueError("drafts must be contiguous int64")
-    if cu_drafts.dtype != torch.int64 or not cu_drafts.is_contiguous():
-        raise ValueError("cu_drafts must be contiguous int64")
-    if uniforms.dtype != torch.float32 or uniforms.shape != (n,) or not uniforms.is_contiguous():
+        qptr = draft_probs.data_ptr()
+    if not _is_vector(drafts, torch.int64, n) or not _is_vector(cu_drafts, torch.int64, batch + 1):
+        raise ValueError("drafts and cu_drafts must be contiguous int64 vectors")
+    if not _is_vector(uniforms, torch.float32, n):
         raise ValueError(f"uniforms must be contiguous float32 [{n}], got {uniforms.dtype} {tuple(uniforms.shape)}")
-    if final_uniforms.dtype != torch.float32 or final_uniforms.shape != (batch,) or not final_uniforms.is_contiguous():
+    if not _is_vector(final_uniforms, torch.float32, batch):
         raise ValueError(f"final_uniforms must be contiguous float32 [{batch}], got {final_uniforms.dtype} "
                          f"{tuple(final_uniforms.shape)}")
     tptr = None
     if temperature is not None:
-        if temperature.dtype != torch.float32 or temperature.shape != (batch,) or not temperature.is_contiguous():
+        if not _is_vector(temperature, torch.float32, batch):
             raise ValueError(f"temperature must be contiguous float32 [{batch}], got {temperature.dtype} "
                              f"{tuple(temperature.shape)}")
         tptr = temperature.data_ptr()
-    dev = _require_cuda(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature)
-    for t, num, want in ((accepted, batch, torch.int64), (tokens, n + batch, torch.int64),
-                         (log_probs, n + batch, torch.float32)):
-        if t.dtype != want or not t.is_contiguous() or t.numel() != num or t.device != dev:
-            raise ValueError(f"outputs must be contiguous on {dev}: int64 accepted [{batch}], int64 tokens and float32 "
-                             f"log_probs [{n + batch}]")
-    _call("verify_drafts", "frx_verify_drafts", dev, logits.data_ptr(), dt, max(logits.stride(0), vocab),
-          drafts.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), final_uniforms.data_ptr(), qptr, qdt, ldq, tptr,
+    if not (_is_vector(accepted, torch.int64, batch) and _is_vector(tokens, torch.int64, rows)
+            and _is_vector(log_probs, torch.float32, rows)):
+        raise ValueError(f"outputs must be contiguous: int64 accepted [{batch}], int64 tokens and float32 log_probs "
+                         f"[{rows}]")
+    dev = _one_device(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature)
+    _call("verify_drafts", "frx_verify_drafts", dev, logits.data_ptr(), dt, max(ldl, vocab),
+          drafts.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), final_uniforms.data_ptr(), qptr, qdt, max(ldq, vocab), tptr,
           temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
           tokens.data_ptr(), log_probs.data_ptr())

@@ -328,10 +328,12 @@ FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x
 
 /*
  * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
- * HBM: the product's epilogue reduces them to the partials of frx_fwd_partials and frx_finalize merges those,
- * launch_rows rows at a time. Operands as in frx_gemm_i8, target rules as in frx_finalize.
+ * HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
+ * frx_finalize, launch_rows rows at a time (up to 128 rows: all at once). Operands as in frx_gemm_i8, target
+ * rules as in frx_finalize.
  *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
- *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes
+ *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to 128 rows
+ *              16 * ceil(vocab_size / 128) * rows bytes
  * No counterpart in the reference.
  */
 FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_hidden, const float* hidden_scale,
@@ -350,9 +352,9 @@ FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_h
  * sum_{k<=j} w_k > final_uniforms[b] * sum_k w_k, where w = max(p - q, 0) at the rejected draft's row (NULL:
  * p without the rejected token; p itself when nothing is left), or p of the last row after full acceptance.
  * Decisions are taken in 64 bits. T < 1e-6 (or NaN) is greedy: a draft must equal its row's argmax
- * (lowest index of a tie) and the argmax is emitted. T above 1e6 counts as 1e6. NaN logits count as -inf,
- * +inf as the largest float, negative or NaN draft probabilities as 0; a row with nothing left to draw emits
- * -1 with log-probability -inf.
+ * (lowest index of a tie) and the argmax is emitted. T above 1e6 counts as 1e6. NaN logits count as -inf, +inf
+ * as the largest finite float (16-bit logits: the largest bf16 value), negative or NaN draft probabilities
+ * as 0; a row with nothing left to draw emits -1 with log-probability -inf.
  *   logits       [n_drafts + batch, vocab] (dtype BF16, F16 or F32, row stride ld_logits)
  *   drafts       [n_drafts] token ids; one outside [0, vocab) is rejected (FRX_STATUS_BAD_TARGET)
  *   cu_drafts    [batch + 1] non-decreasing from 0; cu_drafts[batch] may be below n_drafts (a padded batch:
@@ -360,7 +362,7 @@ FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_h
  *                bad ones set FRX_STATUS_BAD_OFFSETS
  *   draft_probs  [n_drafts, vocab] (BF16, F16 or F32, row stride ld_draft_probs) or NULL
  *   temperature  [batch] or NULL (then temperature_all)
- *   workspace    at least 4 * (n_drafts + batch) * ceil(vocab / 2048) floats, 16-byte aligned; its contents
+ *   workspace    at least 4 * (n_drafts + batch) * ceil((vocab + 7) / 2048) floats, 16-byte aligned; its contents
  *                need not be kept between calls, and calls that overlap need one each
  *   accepted     [batch] number of accepted drafts
  *   tokens, log_probs  [n_drafts + batch], at the rows of the logits: the emitted tokens and their log p_i

@@ -249,6 +249,13 @@ def test_padded_batch_and_bad_offsets():
         assert ((out[1] >= -1) & (out[1] < 800)).all() or bad == [0, 6, 5]
 
 
+def _same_outcome(a, b):
+    """The same decisions; log_probs of rows that start at other 16-byte offsets are summed in another order, so each
+    is within check()'s bound of the exact value and they are within twice that of each other."""
+    return torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and \
+        bool(((a[2].double() - b[2].double()).abs() <= 2 * (4e-5 + 2.0**-24 * a[2].double().abs())).all())
+
+
 def test_strided_inputs_and_id_types():
     from fast_reduction import verify_drafts
 
@@ -261,12 +268,12 @@ def test_strided_inputs_and_id_types():
         wide_q[:, off:off + 1003] = q
         got = verify_drafts(wide_z[:, off:off + 1003], d.int(), cu.int(), u, r, wide_q[:, off:off + 1003],
                             torch.full((3,), 0.9, device=DEV))
-        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        assert _same_outcome(want, got)
     got = verify_drafts(z.t().contiguous().t(), d, cu, torch.stack([u, u], 1)[:, 0], r, q, 0.9)
-    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert _same_outcome(want, got)
     one = verify_drafts(z[:1].expand(8, 1003), d, cu, u, r, q)  # row stride 0
     ref = verify_drafts(z[:1].repeat(8, 1), d, cu, u, r, q)
-    assert all(torch.equal(a, b) for a, b in zip(one, ref))
+    assert _same_outcome(one, ref)
 
 
 def test_empty_batch():
