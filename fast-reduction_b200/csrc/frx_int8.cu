@@ -563,8 +563,12 @@ struct Int8CEPartialsEpilogue {
 // (the M of the MMA) against all tokens (its N, rounded up to 16), so the padding of the tokens costs nothing in
 // HBM, and two CTAs per SM keep up to 2 x 96 KiB of weight in flight through rings of 128-byte deep K steps.
 // The first ring of weight tiles is requested before the wait for the tokens' quantisation.
+// Against the CTA-pair core (4096 x 128256, us): storing, 1 token 87 : 150, 64 tokens 102 : 112, 128 tokens 122 : 123;
+// scoring, 1 token 98 : 155, 64 tokens 117 : 123, 96 tokens 134 : 123. (The pair's loads of token rows that do
+// not exist are slow.) Hence the two limits.
 constexpr int kFewThreads = 192;
 constexpr int kFewMaxTokens = 128;
+constexpr int kFewMaxScored = 64;
 constexpr int kFewWBytes = 128 * 128;
 constexpr int kFewMaxStages = 6;
 constexpr int kFewRingBytes = 108 * 1024;
@@ -634,16 +638,33 @@ struct FewScore {
     const int token = tid / parts, part = tid % parts;
     const int ncols = min(128, p.op.cols - n0);
     const float* z = zbuf + (token < rows ? token : 0) * pitch;
-    float m = -INFINITY;
-    for (int j = part; j < ncols; j += parts) m = fmaxf(m, z[j]);
-    for (int o = 1; o < parts; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s = 0.0f, u = 0.0f;
-    for (int j = part; j < ncols; j += parts) {
-      const float d = z[j] - m;
-      const float e = ex2_approx(d * kLog2e);
-      s += e;
-      u = fmaf(d, e, u);
+    // eight columns in flight: a column at a time was bound by the latency of shared memory (116 tokens x 855 x
+    // 1653: 24 us)
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    for (int j0 = part; j0 < ncols; j0 += 8 * parts) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i * parts;
+        const float x = j < ncols ? z[j] : -INFINITY;
+        m4[i & 3] = fmaxf(m4[i & 3], x);
+      }
     }
+    float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+    for (int o = 1; o < parts; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = part; j0 < ncols; j0 += 8 * parts) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = j0 + i * parts;
+        if (j < ncols) {
+          const float d = z[j] - m;
+          const float e = ex2_approx(d * kLog2e);
+          s4[i & 3] += e;
+          u4[i & 3] = fmaf(d, e, u4[i & 3]);
+        }
+      }
+    }
+    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]), u = (u4[0] + u4[1]) + (u4[2] + u4[3]);
     for (int o = 1; o < parts; o <<= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, o);
       u += __shfl_xor_sync(0xffffffffu, u, o);
@@ -900,7 +921,7 @@ static int launch_product(const I8Operands& op, void* out, int64_t ld_out, int* 
                                                  stream, op.quantised_here);
 }
 
-// Softmax partials of up to kFewMaxTokens tokens, one per 128 columns.
+// Softmax partials of up to kFewMaxScored tokens, one per 128 columns.
 static int launch_few_score(const I8Operands& op, const int64_t* target, float* partials, int64_t n_tiles, int* status,
                             cudaStream_t stream) {
   FewScore::Params ep = {};
@@ -986,7 +1007,7 @@ extern "C" int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t l
               "frx_i8_ce_entropy: need targets and launch_rows >= 1 (got %lld)", (long long)launch_rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Few tokens go in one launch, whose partials cover 128 columns, whatever launch_rows is.
-  const bool few = rows <= kFewMaxTokens;
+  const bool few = rows <= kFewMaxScored;
   const int64_t tile = few ? 128 : kBN;
   const int64_t n_tiles = vocab_size > 0 ? (vocab_size + tile - 1) / tile : 0;
   const int64_t step = few || launch_rows >= rows ? rows : launch_rows;

@@ -23,6 +23,7 @@
 //           bound by issue slots and the 64-bit pipe (64 lanes per SM and clock), so the exponential is a
 //           short one of its own (exp2_scaled below).
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 #include "frx_epilogue.cuh"
@@ -140,6 +141,25 @@ struct Vec8 {
     const float2 f = unpack2(w[j / 2], std::is_same<T, __half>::value);
     return (j & 1) ? f.y : f.x;
   }
+  // The largest value; NaN is dropped (all NaN: NaN).
+  __device__ __forceinline__ float max() const {
+    if (sizeof(T) == 4)
+      return fmaxf(fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3))), fmaxf(fmaxf(at(4), at(5)), fmaxf(at(6), at(7))));
+    uint32_t m;
+    if (std::is_same<T, __half>::value) {
+      __half2 h[4];
+      memcpy(h, w, sizeof(h));
+      const __half2 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      memcpy(&m, &x, sizeof(m));
+    } else {
+      __nv_bfloat162 h[4];
+      memcpy(h, w, sizeof(h));
+      const __nv_bfloat162 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      memcpy(&m, &x, sizeof(m));
+    }
+    const float2 f = unpack2(m, std::is_same<T, __half>::value);
+    return fmaxf(f.x, f.y);
+  }
   __device__ __forceinline__ void mask(int j) {  // value j becomes -inf
     if (sizeof(T) == 4)
       w[j % kWords] = kNegInf;
@@ -213,11 +233,11 @@ __device__ __forceinline__ void join_stats(RowStats& r, const RowStats& o, float
 // Adds 8 N values to a lane's statistics: those of N vectors 256 columns apart, the first one's column is col.
 template <typename T, int N>
 __device__ __forceinline__ void add_vectors(RowStats& r, const Vec8<T> (&raw)[N], float k, bool greedy, uint32_t col) {
-  float v[8 * N], top = -INFINITY;
+  float v[8 * N], top = raw[0].max();
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, raw[i].max());
 #pragma unroll
   for (int j = 0; j < 8 * N; ++j) v[j] = raw[j / 8].at(j % 8);
-#pragma unroll
-  for (int j = 0; j < 8 * N; j += 2) top = fmaxf(top, fmaxf(v[j], v[j + 1]));  // drops NaN
   float sum;
   auto add = [&]() {
     if (greedy && (top > r.m || (r.s == 0.0f && top == r.m))) {

@@ -43,8 +43,8 @@ def _codes_like(rows: int, cols: int, device: torch.device) -> Tensor:
 
 def _aligned_codes(codes: Tensor) -> Tensor:
     """`codes` itself when its rows start on 16-byte boundaries, else a copy laid out that way."""
-    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= codes.shape[1] \
-            and codes.data_ptr() % 16 == 0:
+    row, unit = codes.stride()
+    if unit == 1 and not row & 15 and row >= codes.shape[1] and not codes.data_ptr() & 15:
         return codes
     out = _codes_like(codes.shape[0], codes.shape[1], codes.device)
     out.copy_(codes)
@@ -55,7 +55,8 @@ def _rows_2d(x: Tensor) -> Tensor:
     """x as a matrix of its rows, with unit column stride and rows that do not overlap."""
     if x.dim() != 2:
         x = x.reshape(x.shape[:-1].numel(), x.shape[-1])
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    row, unit = x.stride()
+    return x if unit == 1 and row >= x.shape[1] else x.contiguous()
 
 
 def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
@@ -83,26 +84,27 @@ def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: O
              hidden_scale: Optional[Tensor]):
     """Operands as the kernels read them, (hidden [M, H], hidden scale [M] or None, weight codes, weight scale, bias);
     what does not concern the layout is checked at the launch (ops)."""
-    if weight_codes.dim() != 2 or weight_codes.dtype != torch.int8:
+    shape = weight_codes.shape
+    if len(shape) != 2 or weight_codes.dtype is not torch.int8:
         raise TypeError(f"weight_codes must be int8 [V, H], got {weight_codes.dtype} {tuple(weight_codes.shape)}")
-    V, H = weight_codes.shape
+    V, H = shape
     if V < 1 or H < 1:
         raise ValueError(f"weight_codes must not be empty, got {tuple(weight_codes.shape)}")
     if H > nat.FRX_I8_MAX_K:
         raise NotImplementedError(f"hidden size {H} > {nat.FRX_I8_MAX_K} could overflow the int32 sums")
-    dims = hidden.dim()
-    if dims < 1 or hidden.shape[-1] != H:
+    shape = hidden.shape
+    if not shape or shape[-1] != H:
         raise ValueError(f"hidden size mismatch: hidden {tuple(hidden.shape)} vs weight_codes {tuple(weight_codes.shape)}")
     _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
     if hidden_scale is not None:
-        if hidden_scale.shape != hidden.shape[:-1]:
-            raise ValueError(f"hidden_scale must be float32 {tuple(hidden.shape[:-1])}, got {hidden_scale.dtype} "
+        if hidden_scale.shape != shape[:-1] or hidden.dtype is not torch.int8:
+            raise ValueError(f"hidden_scale goes with int8 tokens, float32 {tuple(shape[:-1])}; got {hidden_scale.dtype} "
                              f"{tuple(hidden_scale.shape)}")
         hidden_scale = hidden_scale.reshape(-1).contiguous()
     x = _rows_2d(hidden)
-    if hidden.dtype == torch.int8:
+    if hidden_scale is not None:
         x = _aligned_codes(x)
-    if bias is not None:
+    if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     return x, hidden_scale, _aligned_codes(weight_codes), weight_scale.contiguous(), bias
 

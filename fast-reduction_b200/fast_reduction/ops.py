@@ -532,22 +532,27 @@ def i8_workspace_bytes(x: torch.Tensor) -> int:
 def _i8_operands(x, x_scale, weight, weight_scale, bias):
     """Checked operands of an 8-bit product: (device, rows, cols, k, the leading C arguments up to bias_dtype)."""
     xdt = _I8_X_DTYPES.get(x.dtype)
-    if xdt is None or weight.dtype != torch.int8:
+    if xdt is None or weight.dtype is not torch.int8:
         raise TypeError(f"x must be int8, bfloat16, float16 or float32 and weight int8, got {x.dtype} and {weight.dtype}")
     rows, k = x.shape
     cols, wk = weight.shape
     if wk != k:
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
-    if x.stride(1) != 1 or weight.stride(1) != 1:
+    ldx, unit = x.stride()
+    ldw, wunit = weight.stride()
+    if unit != 1 or wunit != 1:
         raise ValueError("x and weight must have unit column stride")
     if not _is_vector(weight_scale, torch.float32, cols):
         raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
                          f"{tuple(weight_scale.shape)}")
+    sptr = None
     if x_scale is None:
-        if x.dtype == torch.int8:
+        if xdt == nat.FRX_DTYPE_I8:
             raise ValueError("int8 tokens need their scales (hidden_scale)")
-    elif x.dtype != torch.int8 or not _is_vector(x_scale, torch.float32, rows):
+    elif xdt != nat.FRX_DTYPE_I8 or not _is_vector(x_scale, torch.float32, rows):
         raise ValueError(f"hidden_scale goes with int8 tokens, contiguous float32 [{rows}]")
+    else:
+        sptr = x_scale.data_ptr()
     bptr, bdt = None, 0
     if bias is not None:
         bdt = _OUT_DTYPES.get(bias.dtype)
@@ -556,8 +561,8 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias):
                              f"{tuple(bias.shape)}")
         bptr = bias.data_ptr()
     dev = _one_device(x, x_scale, weight, weight_scale, bias)
-    return dev, rows, cols, k, (x.data_ptr(), xdt, max(x.stride(0), k), None if x_scale is None else x_scale.data_ptr(),
-                                weight.data_ptr(), max(weight.stride(0), k), weight_scale.data_ptr(), bptr, bdt)
+    return dev, rows, cols, k, (x.data_ptr(), xdt, max(ldx, k), sptr, weight.data_ptr(), max(ldw, k),
+                                weight_scale.data_ptr(), bptr, bdt)
 
 
 def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,

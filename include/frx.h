@@ -329,10 +329,10 @@ FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x
 /*
  * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
  * HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
- * frx_finalize, launch_rows rows at a time (up to 128 rows: all at once). Operands as in frx_gemm_i8, target
+ * frx_finalize, launch_rows rows at a time (up to 64 rows: all at once). Operands as in frx_gemm_i8, target
  * rules as in frx_finalize.
  *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
- *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to 128 rows
+ *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to 64 rows
  *              16 * ceil(vocab_size / 128) * rows bytes
  * No counterpart in the reference.
  */
