@@ -350,6 +350,14 @@ struct Int8StoreEpilogue {
   __device__ __forceinline__ static void finish(const Params&, int) {}
 };
 
+constexpr float kLow = -1e38f;  // below every logit; differences to it stay finite
+
+// The partial of columns none of which is live: empty, or NaN when the sum says that one of them is NaN (maxima drop
+// it, and the merge skips a maximum of -inf).
+__device__ __forceinline__ float4 nothing_live(float s, float zt) {
+  return s == s ? make_float4(-INFINITY, 0.0f, 0.0f, zt) : make_float4(s, s, s, zt);
+}
+
 // Softmax partials of the scaled product, in one pass over the accumulator: thread = token (TMEM lane), 16
 // columns at a time with a running maximum, and s and u rescaled when it rises. A warp has 128 of the tile's
 // 256 columns; the two warps of a token join their statistics through shared memory. Pairs of columns share
@@ -420,8 +428,6 @@ struct Int8CEPartialsEpilogue {
     float m, s, u, zt;
   };
 
-  static constexpr float kLow = -1e38f;  // below every logit; differences to it stay finite
-
   // 16 columns: r are their sums, s_ws their scales (and biases 128 behind them), `lim` of them valid; tcol the
   // target's column among them, or -1.
   template <bool kRagged>
@@ -454,6 +460,12 @@ struct Int8CEPartialsEpilogue {
       for (int i = 0; i < 8; ++i) y[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
     }
     if (tcol >= 0) st.zt = select16(v, tcol);
+    if (kFull) {  // a bias of -inf masks its column: kLow contributes nothing, and -inf times 0 would be NaN
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = v[j] < kLow ? kLow : v[j];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+    }
     float t4[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) t4[q] = fmaxf(fmaxf(v[4 * q], v[4 * q + 1]), fmaxf(v[4 * q + 2], v[4 * q + 3]));
@@ -522,6 +534,10 @@ struct Int8CEPartialsEpilogue {
         columns16<true>(st, r, s_ws + c, ncols - c, xs2, k, k2, (tcol >> 4) == (c >> 4) ? tcol & 15 : -1);
       }
     }
+    if (kFull && st.m <= kLow) {
+      const float4 n = nothing_live(st.s, st.zt);
+      st = {n.x, n.y, n.z, n.w};
+    }
     const float f = kFull ? 1.0f : xs;
     st.m *= f;
     st.u *= f;
@@ -541,14 +557,16 @@ struct Int8CEPartialsEpilogue {
     if (!joined) return false;
     const float4 o = *slot;
     release();
-    if (o.y != 0.0f) {  // the tile reaches into its second half
+    st.zt += o.w;
+    if (st.s == 0.0f) {  // nothing in the first half
+      st = {o.x, o.y, o.z, st.zt};
+    } else if (o.y != 0.0f) {  // something in the second one, which the tile need not reach
       const float top = fmaxf(st.m, o.x);
       const float d0 = st.m - top, d1 = o.x - top;
       const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
       st.u = fmaf(d0, st.s, st.u) * e0 + fmaf(d1, o.y, o.z) * e1;
       st.s = st.s * e0 + o.y * e1;
       st.m = top;
-      st.zt += o.w;
     }
     if (row_ok && device_check(n_blk < p.n_tiles, p.status))
       p.partials[static_cast<int64_t>(n_blk) * p.tile_stride + row] = make_float4(st.m, st.s, st.u, st.zt);
@@ -559,49 +577,81 @@ struct Int8CEPartialsEpilogue {
 };
 
 // ------------------------------------------------------------------------------------ few tokens
-// Up to 128 tokens: the product streams the weight once and is bound by HBM. A CTA owns 128 vocabulary entries
-// (the M of the MMA) against all tokens (its N, rounded up to 16), so the padding of the tokens costs nothing in
-// HBM, and two CTAs per SM keep up to 2 x 96 KiB of weight in flight through rings of 128-byte deep K steps.
-// The first ring of weight tiles is requested before the wait for the tokens' quantisation.
-// Against the CTA-pair core (4096 x 128256, us): storing, 1 token 87 : 150, 64 tokens 102 : 112, 128 tokens 122 : 123;
-// scoring, 1 token 98 : 155, 64 tokens 117 : 123, 96 tokens 134 : 123. (The pair's loads of token rows that do
-// not exist are slow.) Hence the two limits.
-constexpr int kFewThreads = 192;
+// Up to 128 tokens: the product streams the weight once and is bound by HBM. The vocabulary is the M of the MMA and
+// the tokens are its N (rounded up to 16), so the tokens' padding costs nothing in HBM. Two persistent CTAs per SM
+// walk tiles of 128 vocabulary entries: warp 0 keeps the ring of 128-byte deep K steps filled across tiles, warp 1
+// issues the MMAs, and four warps drain the finished one of two accumulators, so neither a tile's start nor its
+// end interrupts the stream (64 tokens x 4096 x 128256: 92 us, 102 us with a CTA per tile; one CTA per SM on 256
+// entries, which reads the tokens half as often, took 96 us). The first ring of weight tiles is requested before
+// the wait for the tokens' quantisation.
+// Against the CTA-pair core, us at 4096 x 128256 and 1024 x 32000 (its loads of token rows that do not exist are slow):
+//   storing   1 token 88 : 145, 12 : 16    64 tokens 96 : 113, 14 : 17    128 tokens 109 : 124, 17 : 19
+//   scoring   1 token 98 : 152, 17 : 23    64 tokens 109 : 125, 21 : 22    128 tokens 136 : 130, 27 : 21
 constexpr int kFewMaxTokens = 128;
 constexpr int kFewMaxScored = 64;
 constexpr int kFewWBytes = 128 * 128;
+constexpr int kFewThreads = 192;
+constexpr int kFewSmemBudget = 115712;  // of 228 KiB per SM for two CTAs, each with 1 KiB for the system
 constexpr int kFewMaxStages = 6;
-constexpr int kFewRingBytes = 108 * 1024;
-constexpr int kFewOtherBytes = 1024 + 4 * 4 * kFewMaxTokens + 256;  // alignment, scales, barriers
 
 inline int few_tokens_padded(int64_t rows) { return static_cast<int>((rows + 15) / 16 * 16); }
-inline int few_stages(int nt) {
-  const int n = kFewRingBytes / (kFewWBytes + nt * 128);
-  return n < kFewMaxStages ? n : kFewMaxStages;
-}
+
+// What an epilogue warp works with: entries 32 q .. 32 q + 31 of a tile.
+struct FewWarp {
+  int tile;
+  int buf;  // accumulator
+  int q, lane;
+  uint32_t tacc;
+  float ws, b;  // scale and bias of this lane's entry
+  const float* s_scale;
+};
 
 // Stores the product.
 template <typename OutT>
 struct FewStore {
   using Params = I8Out;
+  static constexpr int kSmemBytes = 0;
   __device__ __forceinline__ static const I8Out& operands(const Params& p) { return p; }
+  __device__ __forceinline__ static void init(const Params&, uint8_t*, int) {}
 
-  __device__ __forceinline__ static void run(const Params& p, bool good, uint8_t* /*ring*/, const float* s_scale,
-                                             uint32_t tacc, int n0, int q, int lane, float ws, float b, int* /*status*/) {
-    const int j = n0 + q * 32 + lane;
-    if (!good || j - lane >= p.cols) return;
-    float v[32];
+  template <class Release, class Wait>
+  __device__ __forceinline__ static bool run(const Params& p, const FewWarp& w, uint8_t* /*smem*/, uint64_t* /*join*/,
+                                             uint32_t /*parity*/, int* /*status*/, Release release, Wait /*wait*/) {
+    const int j = w.tile * 128 + w.q * 32 + w.lane;
+    if (j - w.lane < p.cols) {
+      float v[32];
 #pragma unroll 1
-    for (int c = 0; c < p.rows; c += 32) {
-      __syncwarp();
-      tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
-      store_tokens32<OutT>(p, v, s_scale + c, j, c, ws, b);
+      for (int c = 0; c < p.rows; c += 32) {
+        __syncwarp();
+        tmem_load_32cols(w.tacc + static_cast<uint32_t>(c), v);
+        store_tokens32<OutT>(p, v, w.s_scale + c, j, c, w.ws, w.b);
+      }
     }
+    release();
+    return true;
   }
 };
 
-// Reduces the product to softmax partials of 128 columns: the logits go to shared memory (the ring, which is free by
-// then), [token][column], and 128 / tokens threads (a power of two, at most 32) take a token each way.
+// After it, lane i holds the reduction of a[i] over the warp's lanes: at each step a lane keeps the half of its values
+// that its number points to and gives the other half away (31 shuffles instead of 160).
+template <class Op>
+__device__ __forceinline__ float reduce_transposed(float (&a)[32], int lane, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < o) {
+        const float keep = up ? a[i + o] : a[i], give = up ? a[i] : a[i + o];
+        a[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      }
+    }
+  }
+  return a[0];
+}
+
+// Reduces the product to softmax partials of 128 columns. A warp reduces its 32 columns for 32 tokens at a time, lane =
+// token after reduce_transposed; the first warp joins the four.
 struct FewScore {
   struct Params {
     I8Out op;  // no output
@@ -610,88 +660,125 @@ struct FewScore {
     int64_t tile_stride;
     int n_tiles;
   };
+  // joins: [accumulator][warps 1 to 3][token]; targets' logits: [warp][token]; targets
+  static constexpr int kJoinBytes = 2 * 3 * kFewMaxScored * 16;
+  static constexpr int kZtBytes = 4 * kFewMaxScored * 4;
+  static constexpr int kSmemBytes = kJoinBytes + kZtBytes + kFewMaxScored * 4;
   __device__ __forceinline__ static const I8Out& operands(const Params& p) { return p.op; }
 
-  __device__ __forceinline__ static void run(const Params& p, bool good, uint8_t* ring, const float* s_scale,
-                                             uint32_t tacc, int n0, int q, int lane, float ws, float b, int* status) {
-    const int rows = p.op.rows;
-    const int tid = q * 32 + lane;
-    int parts = 32;
-    while (parts * rows > 128) parts >>= 1;
-    const int pitch = 128 + parts;  // lanes of a warp fall on different banks
-    float* zbuf = reinterpret_cast<float*>(ring);
-    if (good) {
-      float v[32];
-#pragma unroll 1
-      for (int c = 0; c < rows; c += 32) {
+  // The targets as 32-bit ids (-1: not one of the vocabulary's).
+  __device__ __forceinline__ static void init(const Params& p, uint8_t* smem, int thread) {
+    int* s_target = reinterpret_cast<int*>(smem + kJoinBytes + kZtBytes);
+    if (thread < kFewMaxScored) {
+      const int64_t t = thread < p.op.rows ? p.target[thread] : -1;
+      s_target[thread] = t >= 0 && t < p.op.cols ? static_cast<int>(t) : -1;
+    }
+  }
+
+  template <class Release, class Wait>
+  __device__ __forceinline__ static bool run(const Params& p, const FewWarp& w, uint8_t* smem, uint64_t* join,
+                                             uint32_t parity, int* status, Release release, Wait wait) {
+    const int rows = p.op.rows, lane = w.lane;
+    const int j = w.tile * 128 + w.q * 32 + lane;
+    const bool live = j < p.op.cols;
+    float4* slots = reinterpret_cast<float4*>(smem) + w.buf * 3 * kFewMaxScored;
+    float* s_zt = reinterpret_cast<float*>(smem + kJoinBytes) + w.q * kFewMaxScored;
+    const int* s_target = reinterpret_cast<const int*>(smem + kJoinBytes + kZtBytes);
+    float4 own[kFewMaxScored / 32];
+    auto max2 = [](float x, float y) { return fmaxf(x, y); };
+    auto add2 = [](float x, float y) { return x + y; };
+#pragma unroll
+    for (int g = 0; g < kFewMaxScored / 32; ++g) {
+      const int c = g * 32;
+      if (c < rows) {
+        float v[32], a[32];
         __syncwarp();
-        tmem_load_32cols(tacc + static_cast<uint32_t>(c), v);
+        s_zt[c + lane] = 0.0f;
+        __syncwarp();
+        tmem_load_32cols(w.tacc + static_cast<uint32_t>(c), v);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (c + i < rows)
-            zbuf[(c + i) * pitch + tid] = fmaf(static_cast<float>(__float_as_int(v[i])) * s_scale[c + i], ws, b);
-      }
-    }
-    // all four warps come here, whatever their waits said
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (!good) return;
-    const int token = tid / parts, part = tid % parts;
-    const int ncols = min(128, p.op.cols - n0);
-    const float* z = zbuf + (token < rows ? token : 0) * pitch;
-    // eight columns in flight: a column at a time was bound by the latency of shared memory (116 tokens x 855 x
-    // 1653: 24 us)
-    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    for (int j0 = part; j0 < ncols; j0 += 8 * parts) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + i * parts;
-        const float x = j < ncols ? z[j] : -INFINITY;
-        m4[i & 3] = fmaxf(m4[i & 3], x);
-      }
-    }
-    float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-    for (int o = 1; o < parts; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j0 = part; j0 < ncols; j0 += 8 * parts) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = j0 + i * parts;
-        if (j < ncols) {
-          const float d = z[j] - m;
-          const float e = ex2_approx(d * kLog2e);
-          s4[i & 3] += e;
-          u4[i & 3] = fmaf(d, e, u4[i & 3]);
+        for (int i = 0; i < 32; ++i) {
+          v[i] = fmaf(static_cast<float>(__float_as_int(v[i])) * w.s_scale[c + i], w.ws, w.b);
+          if (s_target[c + i] == j) s_zt[c + i] = v[i];
+          v[i] = v[i] < kLow ? kLow : v[i];  // a bias of -inf masks its column
+          a[i] = live ? v[i] : -INFINITY;
         }
+        const float m = reduce_transposed(a, lane, max2);
+        float u[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float d = v[i] - __shfl_sync(0xffffffffu, m, i);
+          const float e = ex2_approx(d * kLog2e);
+          a[i] = live ? e : 0.0f;
+          u[i] = live ? d * e : 0.0f;
+        }
+        const float s = reduce_transposed(a, lane, add2);
+        const float us = reduce_transposed(u, lane, add2);
+        __syncwarp();
+        own[g] = make_float4(m, s, us, s_zt[c + lane]);
+        if (m <= kLow) own[g] = nothing_live(s, own[g].w);
+        if (w.q != 0) slots[(w.q - 1) * kFewMaxScored + c + lane] = own[g];
       }
     }
-    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]), u = (u4[0] + u4[1]) + (u4[2] + u4[3]);
-    for (int o = 1; o < parts; o <<= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      u += __shfl_xor_sync(0xffffffffu, u, o);
+    if (w.q != 0) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&join[w.buf]);
+      release();
+      return true;
     }
-    const int tile = n0 >> 7;
-    if (token < rows && part == 0 && device_check(tile < p.n_tiles, status)) {
-      const int64_t t = p.target[token] - n0;
-      p.partials[tile * p.tile_stride + token] = make_float4(m, s, u, t >= 0 && t < ncols ? z[t] : 0.0f);
+    // the others write these slots again only for the accumulator's next tile, which waits for this release
+    if (!wait(&join[w.buf], parity)) return false;
+#pragma unroll
+    for (int g = 0; g < kFewMaxScored / 32; ++g) {
+      const int token = g * 32 + lane;
+      if (g * 32 < rows) {
+        float4 t = own[g];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          const float4 o = slots[k * kFewMaxScored + token];
+          t.w += o.w;
+          if (o.y == 0.0f) continue;  // nothing there
+          if (t.y == 0.0f) {
+            t = make_float4(o.x, o.y, o.z, t.w);
+            continue;
+          }
+          const float top = fmaxf(t.x, o.x);
+          const float d0 = t.x - top, d1 = o.x - top;
+          const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
+          t.z = fmaf(d0, t.y, t.z) * e0 + fmaf(d1, o.y, o.z) * e1;
+          t.y = t.y * e0 + o.y * e1;
+          t.x = top;
+        }
+        if (token < rows && w.tile * 128 < p.op.cols && device_check(w.tile < p.n_tiles, status))
+          p.partials[w.tile * p.tile_stride + token] = t;
+      }
     }
+    release();
+    return true;
   }
 };
 
 template <class Epi>
 __global__ void __launch_bounds__(kFewThreads, 2)
     gemm_i8_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
-                       const __grid_constant__ typename Epi::Params ep, int nt, int num_k, int stages, int* status) {
+                       const __grid_constant__ typename Epi::Params ep, int nt, int num_k, int stages, int num_tiles,
+                       int* status) {
   const I8Out& p = Epi::operands(ep);
   grid_dep_launch();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int w_bytes = kFewWBytes;
   const int x_bytes = nt * 128;
   uint8_t* s_w = smem;
-  uint8_t* s_x = smem + stages * kFewWBytes;
+  uint8_t* s_x = smem + stages * w_bytes;
   float* s_scale = reinterpret_cast<float*>(s_x + stages * x_bytes);  // the tokens', per epilogue warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + 4 * kFewMaxTokens);
+  uint8_t* s_epi = reinterpret_cast<uint8_t*>(s_scale + 4 * kFewMaxTokens);
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_epi + Epi::kSmemBytes);
   uint64_t* empty = full + kFewMaxStages;
-  uint64_t* done = empty + kFewMaxStages;
+  uint64_t* acc_full = empty + kFewMaxStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* join = acc_empty + 2;  // per accumulator
+  uint64_t* done = join + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   if (!device_check(reinterpret_cast<const uint8_t*>(tmem_slot + 2) - smem_raw <=
@@ -699,12 +786,17 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                     threadIdx.x == 0 ? status : nullptr))
     return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = static_cast<int>(blockIdx.x) * 128;
-  const uint32_t tmem_cols = nt <= 32 ? 32u : (nt <= 64 ? 64u : 128u);
+  const uint32_t acc_cols = nt <= 32 ? 32u : (nt <= 64 ? 64u : 128u);
+  const uint32_t tmem_cols = 2 * acc_cols;
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+      mbar_init(&join[b], 3);
     }
     mbar_init(done, 1);
     *abort_flag = 0;
@@ -718,37 +810,51 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     tmem_alloc(tmem_slot, tmem_cols);
     tmem_relinquish();
   }
+  if (warp >= 2) Epi::init(ep, s_epi, threadIdx.x - 64);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int my_tiles = (num_tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) /
+                       static_cast<int>(gridDim.x);  // tiles blockIdx.x, blockIdx.x + gridDim.x, ...
 
   if (warp == 0) {
     if (lane == 0) {
-      const int pre = num_k < stages ? num_k : stages;
-      for (int kb = 0; kb < pre; ++kb) {
-        mbar_arrive_expect_tx(&full[kb], static_cast<uint32_t>(kFewWBytes + x_bytes));
-        tma_load_2d(s_w + kb * kFewWBytes, &tm_w, &full[kb], kb * 128, n0);
-      }
+      const long long total = static_cast<long long>(my_tiles) * num_k;
+      const int pre = static_cast<int>(total < stages ? total : stages);
+      // K steps in order, over all tiles: w and x are asked for in step `it` of stage it % stages
+      int tile = static_cast<int>(blockIdx.x), kb = 0;
+      auto load_w = [&](int stage) {
+        mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(w_bytes + x_bytes));
+        tma_load_2d(s_w + stage * w_bytes, &tm_w, &full[stage], kb * 128, tile * 128);
+      };
+      auto next_step = [&]() {
+        if (++kb == num_k) {
+          kb = 0;
+          tile += static_cast<int>(gridDim.x);
+        }
+      };
+      for (int s = 0; s < pre; ++s, next_step()) load_w(s);
       grid_dep_wait();
-      for (int kb = 0; kb < pre; ++kb) tma_load_2d(s_x + kb * x_bytes, &tm_x, &full[kb], kb * 128, 0);
+      for (int s = 0; s < pre; ++s) tma_load_2d(s_x + s * x_bytes, &tm_x, &full[s], (s % num_k) * 128, 0);
       int stage = 0;
       uint32_t phase = 0;  // of empty[stage] to wait for
-      int kb = pre;
-      for (; kb < num_k; ++kb) {
-        if (!mbar_wait_bounded(&empty[stage], phase, abort_flag, status, kStatusTimeoutProducer)) break;
-        mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(kFewWBytes + x_bytes));
-        tma_load_2d(s_w + stage * kFewWBytes, &tm_w, &full[stage], kb * 128, n0);
+      long long it = pre;
+      for (; it < total; ++it, next_step()) {
+        if (!mbar_wait_bounded(&empty[stage], phase, abort_flag, status, kStatusTimeoutProducer, kWaitLimitNs,
+                               kSuspendHintShortNs))
+          break;
+        load_w(stage);
         tma_load_2d(s_x + stage * x_bytes, &tm_x, &full[stage], kb * 128, 0);
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      if (kb < num_k) {
+      if (it < total) {
         // gave up: let every copy still in flight land before the shared memory goes away
-        for (int j = kb > stages ? kb - stages : 0; j < kb; ++j)
-          mbar_wait_drain(&full[j % stages], static_cast<uint32_t>((j / stages) & 1), status);
+        for (long long i = it > stages ? it - stages : 0; i < it; ++i)
+          mbar_wait_drain(&full[i % stages], static_cast<uint32_t>((i / stages) & 1), status);
       }
     }
   } else if (warp == 1) {
@@ -756,43 +862,82 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       const uint32_t idesc = make_idesc_i8(128, nt);
       int stage = 0;
       uint32_t phase = 0;
-      for (int kb = 0; kb < num_k; ++kb) {
-        if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma)) break;
+      bool ok = true;
+      for (int i = 0; i < my_tiles && ok; ++i) {
+        const int buf = i & 1;
+        if (!mbar_wait_bounded(&acc_empty[buf], static_cast<uint32_t>((i >> 1) & 1) ^ 1u, abort_flag, status,
+                               kStatusTimeoutMma, kWaitLimitNs, kSuspendHintShortNs))
+          break;
         tc_fence_after();
-        const uint32_t w_addr = smem_u32(s_w + stage * kFewWBytes);
-        const uint32_t x_addr = smem_u32(s_x + stage * x_bytes);
+        for (int kb = 0; kb < num_k; ++kb) {
+          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma, kWaitLimitNs,
+                                 kSuspendHintShortNs)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t w_addr = smem_u32(s_w + stage * w_bytes);
+          const uint32_t x_addr = smem_u32(s_x + stage * x_bytes);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_i8(tmem, make_smem_desc_sw128(w_addr + k * 32, 16, 1024), make_smem_desc_sw128(x_addr + k * 32, 16, 1024),
-                  idesc, (kb | k) != 0 ? 1u : 0u);
-        umma_commit(&empty[stage]);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
+          for (int k = 0; k < 4; ++k)
+            umma_i8(tmem + buf * acc_cols, make_smem_desc_sw128(w_addr + k * 32, 16, 1024),
+                    make_smem_desc_sw128(x_addr + k * 32, 16, 1024), idesc, (kb | k) != 0 ? 1u : 0u);
+          umma_commit(&empty[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
+        if (ok) umma_commit(&acc_full[buf]);
       }
       umma_commit(done);
       mbar_wait_drain(done, 0, status);  // before TMEM is released
     }
     __syncwarp();
   } else {
-    const int q = warp & 3;
-    const int j = n0 + q * 32 + lane;
-    const bool ok = j < p.cols;
-    const float ws = ok ? __ldg(p.col_scale + j) : 0.0f;
-    const float b = ok && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, j) : 0.0f;
+    FewWarp w;
+    w.q = warp & 3;
+    w.lane = lane;
+    auto entry = [&](int i, float& ws, float& b) {  // of the i-th tile
+      const int tile = static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x);
+      const int j = tile * 128 + w.q * 32 + lane;
+      const bool ok = j < p.cols;
+      ws = ok ? __ldg(p.col_scale + j) : 0.0f;
+      b = ok && p.bias != nullptr ? bias_at(p.bias, p.bias_dtype, j) : 0.0f;
+    };
+    float ws = 0.0f, b = 0.0f;
+    entry(0, ws, b);
     grid_dep_wait();
-    float* s = s_scale + q * kFewMaxTokens;
+    float* s = s_scale + w.q * kFewMaxTokens;
 #pragma unroll
     for (int i = 0; i < kFewMaxTokens; i += 32)
       if (i < p.rows) s[i + lane] = i + lane < p.rows ? ld_dep_f32(p.row_scale + i + lane) : 0.0f;
     __syncwarp();
-    int good = 1;
-    if (lane == 0)
-      good = mbar_wait_bounded(done, 0, abort_flag, status, kStatusTimeoutEpilogue) && *abort_flag == 0 ? 1 : 0;
-    good = __shfl_sync(0xffffffffu, good, 0);
-    tc_fence_after();
-    Epi::run(ep, good != 0, s_w, s, tmem + (static_cast<uint32_t>(q * 32) << 16), n0, q, lane, ws, b, status);
+    w.s_scale = s;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      int good = 1;
+      if (lane == 0)
+        good = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, kWaitLimitNs,
+                                 kSuspendHintShortNs);
+      return __shfl_sync(0xffffffffu, good, 0) != 0;
+    };
+    for (int i = 0; i < my_tiles; ++i) {
+      w.buf = i & 1;
+      const uint32_t parity = static_cast<uint32_t>((i >> 1) & 1);
+      w.ws = ws;
+      w.b = b;
+      if (i + 1 < my_tiles) entry(i + 1, ws, b);  // requested under this tile
+      if (!wait(&acc_full[w.buf], parity)) break;
+      tc_fence_after();
+      w.tile = static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x);
+      w.tacc = tmem + w.buf * acc_cols + (static_cast<uint32_t>(w.q * 32) << 16);
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[w.buf]);
+      };
+      if (!Epi::run(ep, w, s_epi, join, parity, status, release, wait)) break;
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -896,7 +1041,11 @@ static int prepare_i8(const char* what, const void* x, int x_dtype, int64_t ld_x
 template <class Epi>
 static int launch_few(const I8Operands& op, const typename Epi::Params& ep, int* status, cudaStream_t stream) {
   const int nt = few_tokens_padded(op.rows);
-  const int stages = few_stages(nt);
+  // alignment, the tokens' scales, the epilogue's, barriers
+  constexpr int kOther = 1024 + 4 * kFewMaxTokens * 4 + Epi::kSmemBytes + 256;
+  const int stage_bytes = kFewWBytes + nt * 128;
+  const int fit = (kFewSmemBudget - kOther) / stage_bytes;
+  const int stages = fit < kFewMaxStages ? fit : kFewMaxStages;
   CUtensorMap tm_w, tm_x;
   int rc = encode_8bit_2d(&tm_w, op.w, op.cols, op.k, op.ld_w, 128, 128);
   if (rc) return rc;
@@ -904,12 +1053,15 @@ static int launch_few(const I8Operands& op, const typename Epi::Params& ep, int*
   if (rc) return rc;
   static std::atomic<uint64_t> attr_done{0};
   auto kernel = gemm_i8_few_kernel<Epi>;
-  constexpr int kMaxSmem = kFewRingBytes + kFewOtherBytes;
-  rc = ensure_smem_attr(kernel, attr_done, kMaxSmem);
+  rc = ensure_smem_attr(kernel, attr_done, kFewSmemBudget);
   if (rc) return rc;
-  const int smem = stages * (kFewWBytes + nt * 128) + kFewOtherBytes;
-  return launch_kernel(kernel, static_cast<unsigned>((op.cols + 127) / 128), kFewThreads, smem, stream,
-                       op.quantised_here, tm_w, tm_x, ep, nt, static_cast<int>((op.k + 127) / 128), stages, status);
+  int sms = 0;
+  rc = sm_count(&sms);
+  if (rc) return rc;
+  const int num_tiles = static_cast<int>((op.cols + 127) / 128);
+  return launch_kernel(kernel, static_cast<unsigned>(num_tiles < 2 * sms ? num_tiles : 2 * sms), kFewThreads,
+                       stages * stage_bytes + kOther, stream, op.quantised_here, tm_w, tm_x, ep, nt,
+                       static_cast<int>((op.k + 127) / 128), stages, num_tiles, status);
 }
 
 template <typename OutT>

@@ -314,3 +314,54 @@ def test_zero_negative_and_uneven_scales(rows):
         ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, t)
         assert ((ce.double() - ce_r).abs() <= tol_ce).all()
         assert ((ent.double() - ent_r).abs() <= tol_ent).all()
+
+
+@pytest.mark.parametrize("rows", [3, 64, 65, 300])
+@pytest.mark.parametrize("v", [97, 513, 3000])
+def test_bias_of_minus_infinity_masks_its_column(rows, v):
+    """Masked vocabulary entries take no part in CE and entropy; a masked target has CE +inf; a row whose mask leaves
+    nothing has NaN."""
+    from fast_reduction import int8_ce_entropy, int8_linear
+
+    x, w, ws, b = make(rows, 96, v, torch.float32, rows + v, torch.float32)
+    masked = torch.rand(v, device=DEV, generator=_gen(1)) < 0.5
+    masked[0], masked[v - 1] = False, True
+    if v > 600:
+        masked[256:512] = True  # a whole tile, and half of another
+        masked[640:768] = True
+    b[masked] = -float("inf")
+    t = torch.randint(0, v, (rows,), device=DEV, generator=_gen(2))
+    t[0] = 0
+    ce, ent, lp = int8_ce_entropy(x, w, ws, t, bias=b)
+    c, s = ref_quantize(x)
+    keep = ~masked
+    z, mag = ref_logits(c, s, w[keep], ws[keep], b[keep])
+    at = torch.cumsum(keep, 0)[t] - 1
+    ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, at)
+    hit = masked[t]
+    assert (ce[hit] == float("inf")).all() and (lp[hit] == -float("inf")).all()
+    assert ((ce.double() - ce_r).abs() <= tol_ce)[~hit].all()
+    assert ((ent.double() - ent_r).abs() <= tol_ent).all()
+    y = int8_linear(x, w, ws, bias=b)
+    assert (y[:, masked] == -float("inf")).all() and y[:, keep].isfinite().all()
+    b.fill_(-float("inf"))
+    ce, ent, _ = int8_ce_entropy(x, w, ws, t, bias=b)
+    assert ce.isnan().all() and ent.isnan().all()
+
+
+@pytest.mark.parametrize("bias", [None, torch.float32])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_nan_in_the_last_column_alone_in_its_warp(rows, bias):
+    from fast_reduction import int8_ce_entropy
+
+    for v in (97, 129, 257, 385):
+        x, w, ws, b = make(rows, 64, v, torch.bfloat16, v, bias)
+        t = torch.zeros(rows, device=DEV, dtype=torch.int64)
+        ws[v - 1] = float("nan")
+        ce, ent, _ = int8_ce_entropy(x, w, ws, t, bias=b)
+        assert ce.isnan().all() and ent.isnan().all()
+        x2, w2, ws2, _ = make(rows, 64, v, torch.bfloat16, v, bias)
+        x2[1, 3] = float("nan")
+        ce, ent, _ = int8_ce_entropy(x2, w2, ws2, t, bias=b)
+        other = [r for r in range(rows) if r != 1]
+        assert ce[1].isnan() and ent[1].isnan() and ce[other].isfinite().all() and ent[other].isfinite().all()
