@@ -70,11 +70,13 @@ def verify_drafts(
     Returns (accepted int64 [B], tokens int64 [N + B], log_probs fp32 [N + B]): at the logits rows, the tokens
     emitted there and their log p_i (greedy: at temperature 1); -1 and 0 where nothing is emitted. A row that
     leaves nothing to draw emits -1 with log-probability -inf. Decisions are taken in 64 bits. No host
-    synchronisation; nothing is differentiable."""
+    synchronisation. Nothing here is differentiable: logits or draft_probs that require a gradient are refused while
+    gradients are enabled."""
     drafts, cu = _ids(draft_tokens, "draft_tokens"), _ids(cu_drafts, "cu_drafts")
     n, batch = drafts.numel(), cu.numel() - 1
     if batch < 0:
         raise ValueError("cu_drafts must hold at least one offset")
+    ops.refuse_grad("verify_drafts", target_logits, draft_probs)
     logits = _rows(target_logits, "target_logits")
     rows, vocab = logits.shape
     if rows != n + batch or vocab < 1 or (batch == 0 and n):

@@ -29,13 +29,6 @@ from . import ops
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _no_grad_inputs(*tensors: Optional[Tensor]) -> None:
-    for t in tensors:
-        if t is None or not t.requires_grad or not torch.is_grad_enabled():
-            continue
-        raise NotImplementedError("the int8 head has no gradient: call it under torch.no_grad() or on detached tensors")
-
-
 def _codes_like(rows: int, cols: int, device: torch.device) -> Tensor:
     """Uninitialised [rows, cols] int8 codes whose rows start on 16-byte boundaries."""
     return torch.empty(rows, ops.round_up(max(cols, 1), 16), device=device, dtype=torch.int8)[:, :cols]
@@ -71,7 +64,7 @@ def quantize_int8(x: Tensor) -> Tuple[Tensor, Tensor]:
         raise TypeError(f"quantize_int8 takes bfloat16, float16 or float32, got {x.dtype}")
     if x.dim() < 1:
         raise ValueError("quantize_int8 needs at least one dimension")
-    _no_grad_inputs(x)
+    ops.refuse_grad("quantize_int8", x)
     ops._require_cuda(x)
     rows = _rows_2d(x) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
     codes = _codes_like(rows.shape[0], rows.shape[1], x.device)
@@ -95,7 +88,7 @@ def _prepare(hidden: Tensor, weight_codes: Tensor, weight_scale: Tensor, bias: O
     shape = hidden.shape
     if not shape or shape[-1] != H:
         raise ValueError(f"hidden size mismatch: hidden {tuple(hidden.shape)} vs weight_codes {tuple(weight_codes.shape)}")
-    _no_grad_inputs(hidden, weight_scale, bias, hidden_scale)
+    ops.refuse_grad("the int8 head", hidden, weight_scale, bias, hidden_scale)
     if hidden_scale is not None:
         if hidden_scale.shape != shape[:-1] or hidden.dtype is not torch.int8:
             raise ValueError(f"hidden_scale goes with int8 tokens, float32 {tuple(shape[:-1])}; got {hidden_scale.dtype} "

@@ -504,6 +504,13 @@ def _one_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device
     return _require_cuda(first, *rest)
 
 
+def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where a result without a gradient would silently end the graph of one of the inputs."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
 def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
     return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 

@@ -365,3 +365,52 @@ def test_nan_in_the_last_column_alone_in_its_warp(rows, bias):
         ce, ent, _ = int8_ce_entropy(x2, w2, ws2, t, bias=b)
         other = [r for r in range(rows) if r != 1]
         assert ce[1].isnan() and ent[1].isnan() and ce[other].isfinite().all() and ent[other].isfinite().all()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values in, and more than 2^31 logits out: the last rows lie behind offsets of 32 bits."""
+    from fast_reduction import int8_linear, quantize_int8
+
+    rows, k = 140000, 16384  # 2.3e9 values, 4.6 GB
+    x = torch.zeros(rows, k, device=DEV, dtype=torch.bfloat16)
+    last = torch.randn(50, k, device=DEV, generator=_gen(3)).to(torch.bfloat16)
+    x[-50:] = last
+    codes, scale = quantize_int8(x)
+    c, s = ref_quantize(last)
+    assert torch.equal(codes[-50:].double(), c) and torch.equal(scale[-50:], s)
+    assert (scale[:-50] == 0).all() and int(codes[-51].abs().max()) == 0
+    del x, codes, scale
+    v, m = 131072, 17000  # 2.2e9 logits
+    x, w, ws, _ = make(m, 64, v, torch.bfloat16, 1)
+    y = int8_linear(x, w, ws)
+    c, s = ref_quantize(x[-40:])
+    assert_logits(y[-40:], *ref_logits(c, s, w, ws, None))
+    assert torch.equal(y[-40:], int8_linear(x[-40:], w, ws))
+
+
+def test_two_threads_at_once():
+    """Two host threads, each on its own stream, get what serial calls get."""
+    import threading
+
+    from fast_reduction import int8_ce_entropy, int8_linear
+
+    work = [make(rows, 512, 3000, torch.bfloat16, rows) for rows in (20, 200)]
+    t = [torch.randint(0, 3000, (x.shape[0],), device=DEV, generator=_gen(2)) for x, _, _, _ in work]
+    want = [(int8_linear(x, w, ws), int8_ce_entropy(x, w, ws, tt)) for (x, w, ws, _), tt in zip(work, t)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        x, w, ws, _ = work[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                y, sc = int8_linear(x, w, ws), int8_ce_entropy(x, w, ws, t[i])
+                if not (torch.equal(y, want[i][0]) and all(torch.equal(a, b) for a, b in zip(sc, want[i][1]))):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(120)
+    assert not bad

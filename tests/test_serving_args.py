@@ -149,6 +149,10 @@ def test_verify_refusals():
         call(target_logits=z.double())
     with pytest.raises(ValueError, match="column"):
         call(target_logits=z[:, :0], draft_probs=None)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        call(target_logits=z.clone().requires_grad_(True))
+    with pytest.raises(NotImplementedError, match="gradient"):
+        call(draft_probs=q.clone().requires_grad_(True))
     with pytest.raises(ValueError, match="uniforms"):
         call(uniforms=u[:2])
     with pytest.raises(ValueError, match="final_uniforms"):
