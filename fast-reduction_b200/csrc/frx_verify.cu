@@ -240,11 +240,6 @@ __device__ __forceinline__ void add_vectors(RowStats& r, const Vec8<T> (&raw)[N]
   for (int j = 0; j < 8 * N; ++j) v[j] = raw[j / 8].at(j % 8);
   float sum;
   auto add = [&]() {
-    if (greedy && (top > r.m || (r.s == 0.0f && top == r.m))) {
-#pragma unroll
-      for (int j = 8 * N - 1; j >= 0; --j)
-        if (v[j] == top) r.idx = col + (j / 8) * 256 + j % 8;
-    }
     const float m = fmaxf(r.m, top), was = r.s * ex2_approx((r.m - m) * k);
     const uint64_t neg = pack_f32x2(-m, -m), k2 = pack_f32x2(k, k);
     uint64_t s2 = 0, s3 = 0;
@@ -262,6 +257,11 @@ __device__ __forceinline__ void add_vectors(RowStats& r, const Vec8<T> (&raw)[N]
     unpack_f32x2(add_f32x2(s2, s3), f0, f1);
     sum = f0 + f1;
     if (sum <= 8.5f * N) {
+      if (greedy && (top > r.m || (r.s == 0.0f && top == r.m))) {
+#pragma unroll
+        for (int j = 8 * N - 1; j >= 0; --j)
+          if (v[j] == top) r.idx = col + (j / 8) * 256 + j % 8;
+      }
       r.s = was + sum;
       r.m = m;
     }

@@ -353,3 +353,16 @@ def test_head_product_verification_and_scores_together():
         want = reference(z, fresh[1], cu, fresh[2], fresh[3], fresh[4], [1.0] * b)
         assert acc.tolist() == want[0].tolist() and tok.tolist() == want[1].tolist()
         assert ((lp - score).abs() <= 3.1e-5 + 4e-5 + 1.4e-4).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_greedy_takes_the_first_of_several_infinities(dtype):
+    """+inf counts as one finite value, so several tie, also where one thread reads them one after the other."""
+    z, d, cu, u, r, _ = make([2, 1, 0], 9001, dtype, 21, probs=None)
+    for row, cols in enumerate([[5, 1029, 2053], [2047, 2048], [8999, 4104, 8200], [7, 8], [1024, 0], [3, 515, 4611]]):
+        z[row, cols] = float("inf")
+    first = torch.tensor([5, 2047, 4104, 7, 0, 3], device=DEV)
+    d = first[torch.tensor([0, 1, 3], device=DEV)].clone()
+    d[1] = 2048
+    accepted, tokens, _ = check(z, d, cu, u, r, temps=0.0)
+    assert accepted.tolist() == [1, 1, 0] and tokens.tolist() == [5, 2047, -1, 7, 0, 3]
