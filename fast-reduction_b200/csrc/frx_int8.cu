@@ -7,7 +7,7 @@
 //   frx_i8_ce_entropy    the same product reduced to softmax partials (m, s, u, zt) by the epilogue, and
 //                        those to cross-entropy, entropy and log-probability per row
 //
-// |code| <= 127, so a sum over K <= 131072 products stays below 2^31: the int32 accumulators of
+// |code| <= 128, so a sum over K <= 131071 products stays below 2^31: the int32 accumulators of
 // kind::i8 hold it exactly and the result does not depend on the order of the products.
 #include <cstring>
 #include <type_traits>
@@ -17,7 +17,7 @@
 
 namespace frx {
 
-constexpr int64_t kI8MaxK = 131072;
+constexpr int64_t kI8MaxK = 131071;
 
 // ------------------------------------------------------------------------------------ quantisation
 // Eight consecutive values of a row as they lie in memory. max_bits folds the bits of |x| into a running

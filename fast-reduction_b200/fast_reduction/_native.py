@@ -47,7 +47,7 @@ FRX_STATUS_DRAIN_TIMEOUT = 16
 FRX_STATUS_CHECK_FAILED = 32
 FRX_STATUS_BAD_OFFSETS = 64
 
-FRX_I8_MAX_K = 131072  # longest row of 8-bit codes whose products cannot overflow an int32 sum
+FRX_I8_MAX_K = 131071  # longest row of 8-bit codes whose products cannot overflow an int32 sum
 FRX_I8_FEW_ROWS = 64  # up to so many rows frx_i8_ce_entropy makes one partial per 128 columns
 FRX_VERIFY_CHUNK = 2048  # columns per workspace entry of frx_verify_drafts
 

@@ -154,7 +154,7 @@ def int8_ce_entropy(
     """(ce_loss, entropy, log_probs), each fp32 and shaped like ``hidden.shape[:-1]``, of the logits
     int8_linear would give in fp32, which never reach HBM. Operands as in int8_linear; target, chunk_size and
     ignore_index as in gemm_fused_ce_entropy (ignored rows: ce = log_probs = 0, entropy kept; a target
-    outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET)."""
+    outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET). A bias of -inf masks its vocabulary entry."""
     x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
     B = x.shape[0]
     if target.numel() != B:

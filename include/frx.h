@@ -311,8 +311,8 @@ FRX_API int frx_quantize_i8(const void* x, int dtype, int64_t ld_x, int64_t rows
 
 /*
  * out[r, j] = (sum_c xc[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]), with xc and weight [cols, k]
- * signed 8-bit codes within +-127: exact int32 sums (k <= 131072), scaled in fp32 and rounded once to
- * out_dtype (BF16, F16 or F32; any ld_out >= cols and any alignment of the element type).
+ * signed 8-bit codes: exact int32 sums (k <= 131071), scaled in fp32 and rounded once to out_dtype (BF16, F16 or
+ * F32; any ld_out >= cols and any alignment of the element type).
  *   x_dtype    FRX_DTYPE_I8: x holds the codes, x_scale [rows] their scales. FRX_DTYPE_BF16, _F16 or _F32: x is
  *              quantised as by frx_quantize_i8 into the workspace first (x_scale is not read)
  *   codes      16-byte aligned bases, row strides that are multiples of 16
@@ -329,7 +329,8 @@ FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x
 /*
  * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
  * HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
- * frx_finalize, launch_rows rows at a time (up to 64 rows: all at once). Operands as in frx_gemm_i8, target
+ * frx_finalize, launch_rows rows at a time (up to 64 rows: all at once). Logits, and sum * weight_scale, are
+ * expected above -1e38; what is below (a bias of -inf) counts as masked. Operands as in frx_gemm_i8, target
  * rules as in frx_finalize.
  *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
  *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to 64 rows

@@ -148,10 +148,10 @@ def test_linear_matches_64_bits(dtype, out, bias, rows, k, v):
 
 @pytest.mark.parametrize("rows", [1, 30, 400])
 def test_linear_sums_are_exact_at_the_limits(rows):
-    """All codes +-127 over the longest row: the largest sums, which fp32 accumulation could not hold exactly."""
+    """Codes of +-127 and -128 over the longest row: the largest sums, which fp32 accumulation could not hold exactly."""
     from fast_reduction import int8_linear
 
-    k, v = 131072, 200
+    k, v = 131071, 200
     g = _gen(5)
     x = torch.full((rows, k), 127, device=DEV, dtype=torch.int8)
     w = torch.full((v, k), 127, device=DEV, dtype=torch.int8)
@@ -161,6 +161,10 @@ def test_linear_sums_are_exact_at_the_limits(rows):
     y = int8_linear(x, w, torch.ones(v, device=DEV), hidden_scale=one, out_dtype=torch.float32)
     exact = x.double() @ w.double().t()
     assert torch.equal(y, exact.float())
+    x.fill_(-128)
+    w.fill_(-128)
+    y = int8_linear(x, w, torch.ones(v, device=DEV), hidden_scale=one, out_dtype=torch.float32)
+    assert (y == 131071 * 16384).all()
 
 
 def test_linear_operand_layouts():

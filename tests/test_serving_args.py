@@ -38,7 +38,7 @@ def test_product_entry_points(score):
 
     bad = nat.FRX_ERR_INVALID_ARG
     assert call(rows=-1) == bad and call(cols=0) == bad and call(k=0) == bad and call(rows=1 << 31) == bad
-    assert call(k=131073, ld_x=131088, ld_w=131088) == nat.FRX_ERR_UNSUPPORTED
+    assert call(k=131072, ld_x=131072, ld_w=131072) == nat.FRX_ERR_UNSUPPORTED
     assert call(x=None) == bad and call(xs=None) == bad and call(w=None) == bad and call(ws=None) == bad
     assert call(x=A + 8) == bad and call(w=C + 1) == bad and call(ld_x=72) == bad and call(ld_w=48) == bad
     assert call(xdt=4) == bad and call(bias=A, bdt=7) == bad and call(bias=A, bdt=nat.FRX_DTYPE_I8) == bad
@@ -106,7 +106,7 @@ def test_int8_head_refusals():
         with pytest.raises(ValueError, match="hidden_scale"):
             fn(x, w, s, hidden_scale=torch.ones(4))
         with pytest.raises(NotImplementedError, match="overflow"):
-            fn(torch.zeros(1, 131073), torch.zeros(2, 131073, dtype=torch.int8), s[:2])
+            fn(torch.zeros(1, 131072), torch.zeros(2, 131072, dtype=torch.int8), s[:2])
         with pytest.raises(NotImplementedError, match="gradient"):
             fn(x.clone().requires_grad_(True), w, s)
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
