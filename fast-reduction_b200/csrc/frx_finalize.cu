@@ -113,17 +113,19 @@ __global__ void __launch_bounds__(kFinRows* kSplits)
   if (logp != nullptr) logp[row] = -row_ce;
 }
 
-// The merge for frx_i8_ce_entropy, which follows the launch that wrote the partials at once: four times the
-// splits of frx_finalize, so that few rows of many tiles take a quarter of the dependent steps (1024 rows of
-// 125 tiles: 6.8 -> 3 us).
+// The merge for frx_i8_ce_entropy, which follows the launch that wrote the partials at once. With many tiles four times
+// the splits of frx_finalize, so that few rows take a quarter of the dependent steps; with few ones the larger CTA
+// costs more than it spares. The operator's us with 8 and 32 splits: 13 tiles 15.2, 16.3 (427 rows); 5 tiles 22.8,
+// 24.0 (926 rows); 125 tiles 42.2, 40.5 (1024 rows); 397 tiles 37.3, 29.5 (190 rows).
 int launch_finalize_dep(const float* partials, int64_t n_tiles, int64_t rows, int64_t tile_stride,
                         const int64_t* target, int64_t vocab_size, int64_t ignore_index, float* ce, float* entropy,
                         float* lse, float* log_probs, int* status, cudaStream_t stream) {
-  constexpr int kSplits = 32;
-  return launch_kernel(finalize_kernel<kSplits, true>, static_cast<unsigned>((rows + kFinRows - 1) / kFinRows),
-                       kFinRows * kSplits, 0, stream, true, reinterpret_cast<const float4*>(partials), n_tiles, rows,
-                       tile_stride, 0, 0, target, vocab_size, ignore_index, ce, entropy, lse, log_probs,
-                       static_cast<float4*>(nullptr), status);
+  const bool many = n_tiles > 64;
+  return launch_kernel(many ? finalize_kernel<32, true> : finalize_kernel<kFinSplits, true>,
+                       static_cast<unsigned>((rows + kFinRows - 1) / kFinRows), kFinRows * (many ? 32 : kFinSplits), 0,
+                       stream, true, reinterpret_cast<const float4*>(partials), n_tiles, rows, tile_stride, 0, 0,
+                       target, vocab_size, ignore_index, ce, entropy, lse, log_probs, static_cast<float4*>(nullptr),
+                       status);
 }
 
 }  // namespace frx

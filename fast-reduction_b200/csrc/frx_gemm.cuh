@@ -325,7 +325,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
                              int* status) {
   using Cfg = PairCfg<kNH>;
   static_assert(!kI8 || (!kAMN && !kBMN && kNH == 1), "8-bit operands are K-major in 256 x 256 tiles");
-  constexpr uint32_t kHint = kI8 ? kSuspendHintShortNs : kSuspendHintNs;
   constexpr int kSubK = kI8 ? 128 : 64;  // K elements of one 128-byte sub-tile row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -398,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const int n0 = pn * Cfg::kTileN + static_cast<int>(rank) * 128;
         for (int kb = 0; kb < num_k_blocks; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, status, kStatusTimeoutProducer,
-                                 sched.wait_limit_ns, kHint)) {
+                                 sched.wait_limit_ns)) {
             ok = false;
             break;
           }
@@ -473,7 +472,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const int buf = local % Cfg::kNumAcc;
         const uint32_t acc_phase = static_cast<uint32_t>((local / Cfg::kNumAcc) & 1);
         if (!mbar_wait_bounded(&acc_empty[buf], acc_phase ^ 1u, abort_flag, status, kStatusTimeoutMma,
-                               sched.wait_limit_ns, kHint)) {
+                               sched.wait_limit_ns)) {
           ok = false;
           break;
         }
@@ -481,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * 256);
         for (int kb = 0; kb < num_k_blocks; ++kb) {
           if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma,
-                                 sched.wait_limit_ns, kHint)) {
+                                 sched.wait_limit_ns)) {
             ok = false;
             break;
           }
@@ -551,7 +550,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
       int ok = 1;
       if (lane == 0)
         ok = mbar_wait_bounded(&acc_full[buf], acc_phase, abort_flag, status, kStatusTimeoutEpilogue,
-                                   sched.wait_limit_ns, kHint) ? 1 : 0;
+                                   sched.wait_limit_ns) ? 1 : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
@@ -562,7 +561,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         if (lane == 0) {
           const uint32_t bar = map_to_cta(smem_u32(&acc_empty[buf]), 0);
           if (kI8)
-            mbar_arrive_cluster_cta(bar);
+            mbar_arrive_cluster_relaxed(bar);
           else
             mbar_arrive_cluster(bar);
         }
@@ -571,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
         auto wait = [&](uint64_t* bar, uint32_t parity) {
           int done = 1;
           if (lane == 0)
-            done = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, sched.wait_limit_ns, kHint);
+            done = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, sched.wait_limit_ns);
           return __shfl_sync(0xffffffffu, done, 0) != 0;
         };
         if (!Epi::run(ep, tile, s_epi, tacc + static_cast<uint32_t>(half * 128), pm * 2 + static_cast<int>(rank), pn,

@@ -841,8 +841,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       uint32_t phase = 0;  // of empty[stage] to wait for
       long long it = pre;
       for (; it < total; ++it, next_step()) {
-        if (!mbar_wait_bounded(&empty[stage], phase, abort_flag, status, kStatusTimeoutProducer, kWaitLimitNs,
-                               kSuspendHintShortNs))
+        if (!mbar_wait_bounded(&empty[stage], phase, abort_flag, status, kStatusTimeoutProducer))
           break;
         load_w(stage);
         tma_load_2d(s_x + stage * x_bytes, &tm_x, &full[stage], kb * 128, 0);
@@ -866,12 +865,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       for (int i = 0; i < my_tiles && ok; ++i) {
         const int buf = i & 1;
         if (!mbar_wait_bounded(&acc_empty[buf], static_cast<uint32_t>((i >> 1) & 1) ^ 1u, abort_flag, status,
-                               kStatusTimeoutMma, kWaitLimitNs, kSuspendHintShortNs))
+                               kStatusTimeoutMma))
           break;
         tc_fence_after();
         for (int kb = 0; kb < num_k; ++kb) {
-          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma, kWaitLimitNs,
-                                 kSuspendHintShortNs)) {
+          if (!mbar_wait_bounded(&full[stage], phase, abort_flag, status, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
@@ -917,8 +915,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       int good = 1;
       if (lane == 0)
-        good = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, kWaitLimitNs,
-                                 kSuspendHintShortNs);
+        good = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue);
       return __shfl_sync(0xffffffffu, good, 0) != 0;
     };
     for (int i = 0; i < my_tiles; ++i) {
