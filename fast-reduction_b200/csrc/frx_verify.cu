@@ -770,10 +770,16 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
       run += __shfl_sync(0xffffffffu, incl, 31);
     }
     if (token < 0) token = last_live;  // what rounding leaves past the end
+    // The sums say that this group has a live column. Logits that another stream is still writing while they are read
+    // may have none left by now: the token is then -1, and nothing is read before the row.
     if (lane == 0) {
-      const double z = clean_logit<T>(to_f32<T>(static_cast<const T*>(d.z)[token]));
       a.tokens[row] = token;
-      a.log_probs[row] = static_cast<float>((z - rs.m) / st.t - log(static_cast<double>(rs.s)));
+      double logp = -INFINITY;
+      if (token >= 0) {
+        const double z = clean_logit<T>(to_f32<T>(static_cast<const T*>(d.z)[token]));
+        logp = (z - rs.m) / st.t - log(static_cast<double>(rs.s));
+      }
+      a.log_probs[row] = static_cast<float>(logp);
     }
   }
   cluster_sync_all();  // no CTA leaves while another may still read its sums
