@@ -787,13 +787,13 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
   cluster_sync_all();  // no CTA leaves while another may still read its sums
 }
 
-// CTAs per sequence: as many as are resident together (3 per SM), since a second round of clusters costs as much as
-// the first. Sequences with draft probabilities, 0 to 7 drafts each, us with 8, 4, 2 and 1 CTAs:
-//   V = 128256   16: 31, 35    48: 48, 55    64: 64, 58    96: 84, 78
-//   V = 32000    128: -, 41, 36, 40    256: -, 71, 61, 59    512: -, 123, 101, 97
+// CTAs per sequence: many for few sequences, whose columns they share; fewer when the batch fills the GPU anyway,
+// since each CTA of a cluster waits for the decision. Sequences with draft probabilities, us with 8, 4, 2 and 1 CTAs:
+//   V = 128256, 0 to 7 drafts   16: 31, 35    48: 48, 55    64: 55, 57, 63, 92    96: 84, 78
+//   V = 32000, 4 drafts         256: 102, 75, 66, 74
 inline int verify_cluster(int64_t batch, int64_t vocab, int sms) {
   int ctas = kVfyMaxCluster;
-  while (ctas > 1 && (batch * ctas > 3 * sms || vocab <= 256 * kVfyWarps * (ctas / 2))) ctas /= 2;
+  while (ctas > 1 && (batch * ctas > 4 * sms || vocab <= 256 * kVfyWarps * (ctas / 2))) ctas /= 2;
   return ctas;
 }
 
