@@ -15,13 +15,15 @@
 //
 // Two launches:
 //   stats   one warp per (row, 2048 or more columns): max, sum of exp((z - max) / T) and the index of the max.
-//           Reads every logit once: HBM-bound.
+//           Reads every logit once. V = 128256 bf16: 288 rows 19 us (3.9 TB/s), 1150 rows 57 us (5.2 TB/s); exponentials
+//           and loads take turns (a ring of asynchronous copies and smaller or more blocks were no faster).
 //   sample  one cluster of 1 to 8 CTAs per sequence: merges the row statistics, decides a, then draws from
 //           the chosen row. Running sums and probabilities are in 64 bits: which token's interval a
 //           number falls in is a comparison over up to V borders, and sums in 32 bits would move each
 //           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256. It is
 //           bound by issue slots and the 64-bit pipe (64 lanes per SM and clock), so the exponential is a
-//           short one of its own (exp2_scaled below).
+//           short one of its own (exp2_scaled below). 64 sequences of V = 128256 with draft probabilities: 55 us
+//           in all; per cluster 5 us for the decision, 7 for a pass over a row, 3 for the search.
 #include <cmath>
 #include <cstring>
 #include <type_traits>
