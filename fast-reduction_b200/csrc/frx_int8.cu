@@ -12,7 +12,7 @@
 //
 // What bounds them (one B200; 6.56 TB/s is what a copy reaches):
 //   quantisation    HBM: 128256 x 4096 fp32 367 us (7.2 TB/s), bf16 329 us (4.8 TB/s: two dependent phases per row)
-//   few tokens      HBM: 1 token x 4096 x 128256 89 us (5.9 TB/s of weight), 64 tokens 96 us
+//   few tokens      HBM: 1 token x 4096 x 128256 84 us (6.2 TB/s of weight), 64 tokens 92 us
 //   many tokens     the tensor pipe's power and the L2's bandwidth to the SMs together: a 256 x 256 tile moves
 //                   512 bytes per K and SM pair, 12 TB/s. 4096 tokens x 4096 x 32768 stored 406 us (2.7 POP/s),
 //                   x 128256 scored 1.44 ms (3.0 POP/s, tensor pipe 90 % active at 1.53 GHz)
@@ -588,18 +588,20 @@ struct Int8CEPartialsEpilogue {
 // the tokens are its N (rounded up to 16), so the tokens' padding costs nothing in HBM. Two persistent CTAs per SM
 // walk tiles of 128 vocabulary entries: warp 0 keeps the ring of 128-byte deep K steps filled across tiles, warp 1
 // issues the MMAs, and four warps drain the finished one of two accumulators, so neither a tile's start nor its
-// end interrupts the stream (64 tokens x 4096 x 128256: 92 us, 102 us with a CTA per tile; one CTA per SM on 256
-// entries, which reads the tokens half as often, took 96 us). The first ring of weight tiles is requested before
-// the wait for the tokens' quantisation.
+// end interrupts the stream (64 tokens x 4096 x 128256: 102 -> 96 us; one CTA per SM on 256 entries, which reads the
+// tokens half as often, took 99). The first ring of weight tiles is requested before the wait for the tokens'
+// quantisation. The ring holds at most 4 steps, 128 KB of weight in flight per SM (1 token: 88.7 us with 6 steps, 84.1
+// with 4, 86 with 3, 97 with 2), and the weight is marked to leave the L2 first, so that the tokens stay
+// (64 tokens: 96 -> 92 us).
 // Against the CTA-pair core, us at 4096 x 128256 and 1024 x 32000 (its loads of token rows that do not exist are slow):
-//   storing   1 token 88 : 145, 12 : 16    64 tokens 96 : 113, 14 : 17    128 tokens 109 : 124, 17 : 19
-//   scoring   1 token 98 : 152, 17 : 23    64 tokens 109 : 125, 21 : 22    128 tokens 136 : 130, 27 : 21
+//   storing   1 token 84 : 145, 11 : 16    64 tokens 92 : 113, 13 : 17     128 tokens 110 : 124, 16 : 19
+//   scoring   1 token 93 : 152, 18 : 23    64 tokens 105 : 125, 21 : 22    128 tokens 136 : 130, 27 : 21
 constexpr int kFewMaxTokens = 128;
 constexpr int kFewMaxScored = 64;
 constexpr int kFewWBytes = 128 * 128;
 constexpr int kFewThreads = 192;
 constexpr int kFewSmemBudget = 115712;  // of 228 KiB per SM for two CTAs, each with 1 KiB for the system
-constexpr int kFewMaxStages = 6;
+constexpr int kFewMaxStages = 4;
 
 inline int few_tokens_padded(int64_t rows) { return static_cast<int>((rows + 15) / 16 * 16); }
 
@@ -831,9 +833,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       const int pre = static_cast<int>(total < stages ? total : stages);
       // K steps in order, over all tiles: w and x are asked for in step `it` of stage it % stages
       int tile = static_cast<int>(blockIdx.x), kb = 0;
+      const uint64_t once = l2_evict_first();  // the weight; the tokens stay in the L2
       auto load_w = [&](int stage) {
         mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(w_bytes + x_bytes));
-        tma_load_2d(s_w + stage * w_bytes, &tm_w, &full[stage], kb * 128, tile * 128);
+        tma_load_2d_hint(s_w + stage * w_bytes, &tm_w, &full[stage], kb * 128, tile * 128, once);
       };
       auto next_step = [&]() {
         if (++kb == num_k) {
