@@ -126,6 +126,7 @@ def int8_linear(
     if out_dtype not in _FLOATS:
         raise TypeError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
     if out is not None:
+        ops.refuse_grad("int8_linear", out)
         rows, V = hidden.shape[:-1].numel(), weight_codes.shape[0]
         if out.dtype != out_dtype or out.shape != (rows, V) or (V > 1 and out.stride(1) != 1) \
                 or (rows > 1 and out.stride(0) < V):

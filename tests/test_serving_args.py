@@ -118,6 +118,8 @@ def test_int8_head_refusals():
     for out in (torch.zeros(4, 9), torch.zeros(10, 4).t(), torch.zeros(1, 10).expand(4, 10), torch.zeros(3, 10)):
         with pytest.raises(ValueError, match="out must"):
             int8_linear(x, w, s, out=out)
+    with pytest.raises(NotImplementedError, match="gradient"):
+        int8_linear(x, w, s, out=torch.zeros(4, 10, requires_grad=True))
 
 
 def test_verify_refusals():
