@@ -36,7 +36,10 @@ __device__ __forceinline__ RowStat merge_stats(RowStat a, const RowStat& b) {
   const float m_hi = a_hi ? a.m : b.m, m_lo = a_hi ? b.m : a.m;
   const float s_hi = a_hi ? a.s : b.s, s_lo = a_hi ? b.s : a.s;
   const float u_hi = a_hi ? a.u : b.u, u_lo = a_hi ? b.u : a.u;
-  const float d = m_lo - m_hi;  // <= 0
+  // d <= 0. Below -1e4 the lower side adds nothing; its d is held there, so that d * s_lo stays finite behind a mask of
+  // large finite logits (-1e37) and infinity times an e of 0 does not turn up as NaN. NaN stays NaN.
+  float d = m_lo - m_hi;
+  d = d < -1e4f ? -1e4f : d;
   const float e = ex2_approx(d * kLog2e);
   RowStat r;
   r.m = m_hi;

@@ -496,7 +496,9 @@ struct Int8CEPartialsEpilogue {
       s2[i & 1] = add_f32x2(s2[i & 1], e);
       u2[i & 1] = fma_f32x2(dd, e, u2[i & 1]);
     }
-    st.u = fmaf(d, st.s, st.u) * e0;
+    // d * e0 first: columns behind a mask (or with logits of -1e37) leave a d whose product with s passes the
+    // largest float, and infinity times an e0 of 0 would be NaN
+    st.u = fmaf(d * e0, st.s, st.u * e0);
     st.s *= e0;
     st.m = top;
     float f0, f1;
@@ -571,7 +573,7 @@ struct Int8CEPartialsEpilogue {
       const float top = fmaxf(st.m, o.x);
       const float d0 = st.m - top, d1 = o.x - top;
       const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
-      st.u = fmaf(d0, st.s, st.u) * e0 + fmaf(d1, o.y, o.z) * e1;
+      st.u = fmaf(d0 * e0, st.s, st.u * e0) + fmaf(d1 * e1, o.y, o.z * e1);  // as in columns16
       st.s = st.s * e0 + o.y * e1;
       st.m = top;
     }
@@ -754,7 +756,7 @@ struct FewScore {
           const float top = fmaxf(t.x, o.x);
           const float d0 = t.x - top, d1 = o.x - top;
           const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
-          t.z = fmaf(d0, t.y, t.z) * e0 + fmaf(d1, o.y, o.z) * e1;
+          t.z = fmaf(d0 * e0, t.y, t.z * e0) + fmaf(d1 * e1, o.y, o.z * e1);  // d * e first: no overflow
           t.y = t.y * e0 + o.y * e1;
           t.x = top;
         }

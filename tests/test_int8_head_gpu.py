@@ -418,3 +418,33 @@ def test_two_threads_at_once():
     for th in threads:
         th.join(120)
     assert not bad
+
+
+@pytest.mark.parametrize("fill", [-float("inf"), torch.finfo(torch.float32).min, -1e37, -3e36])
+@pytest.mark.parametrize("codes", [False, True])
+@pytest.mark.parametrize("rows", [1, 40, 65, 300])
+def test_masked_stretch_before_live_columns(rows, codes, fill):
+    """Stretches of masked entries of every length that the reductions work in (16 columns, 32, a tile's half, whole
+    tiles), each followed by live ones. What is masked has a weight of 0 in 64 bits too; the bounds are those of
+    ref_score over the live entries."""
+    from fast_reduction import int8_ce_entropy
+
+    v = 1600
+    for stretch in ([0, 16], [0, 100], [16, 48], [0, 128], [128, 200], [64, 256], [0, 256], [0, 1040], [0, v - 1]):
+        x, w, ws, b = make(rows, 96, v, torch.float32, rows + stretch[1], torch.float32)
+        masked = torch.zeros(v, device=DEV, dtype=torch.bool)
+        masked[stretch[0]:stretch[1]] = True
+        b[masked] = fill
+        keep = ~masked
+        live = keep.nonzero()[:, 0]
+        t = live[torch.randint(0, len(live), (rows,), device=DEV, generator=_gen(3))]
+        c, s = ref_quantize(x)
+        if codes:
+            ce, ent, lp = int8_ce_entropy(c.to(torch.int8), w, ws, t, bias=b, hidden_scale=s)
+        else:
+            ce, ent, lp = int8_ce_entropy(x, w, ws, t, bias=b)
+        z, mag = ref_logits(c, s, w[keep], ws[keep], b[keep])
+        ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, torch.cumsum(keep, 0)[t] - 1)
+        assert ((ce.double() - ce_r).abs() <= tol_ce).all(), stretch
+        assert ((ent.double() - ent_r).abs() <= tol_ent).all(), stretch
+        assert torch.equal(lp, -ce)
