@@ -405,7 +405,7 @@ struct DrawRow {
   const void* q;
   double m;
   double scale;  // 1024 log2(e) / T: exp((z - m) / T) = 2^((z - m) scale / 1024)
-  float floor;   // logits below have weight 0: m - 680 T, where exp is 4e-296
+  float floor;   // logits below have weight 0: the least float from m - 680 T on, where exp is 4e-296
   int without;  // kDrawWithout: the token taken out, else -1
   int mode;
 };
@@ -573,10 +573,11 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
         s_decision = {acc, r.m, r.s};
         if (s_pass[acc - i0] < 0 && a.status != nullptr) atomicOr(a.status, kStatusBadTarget);
         a.accepted[b] = acc;
-        if (r.s == 0.0f || st.greedy) {  // nothing to draw
-          a.tokens[row0 + acc] = r.s == 0.0f ? -1 : static_cast<int64_t>(r.idx);
-          a.log_probs[row0 + acc] = r.s == 0.0f ? -INFINITY : static_cast<float>(-log(static_cast<double>(r.s)));
-        }
+        // Nothing to draw, or what the draw's own CTA writes over after the cluster's next barrier: should no warp
+        // take the number, which only logits written during the call could cause, the row is defined all the same.
+        const bool none = r.s == 0.0f || !st.greedy;
+        a.tokens[row0 + acc] = none ? -1 : static_cast<int64_t>(r.idx);
+        a.log_probs[row0 + acc] = none ? -INFINITY : static_cast<float>(-log(static_cast<double>(r.s)));
       }
       __syncthreads();
     }
@@ -606,7 +607,9 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
   d.z = logits + row * a.ld_logits;
   d.q = a.q == nullptr ? nullptr : static_cast<const Q*>(a.q) + (lo + acc) * a.ld_q;
   d.m = rs.m;
-  d.floor = rs.m - 680.0f * st.t;
+  // rounded up: at 1500 and T = 1e-6 a step of fp32 is 122 T, and a cutoff rounded down would let in logits below the
+  // range of exp2_scaled, whose results are some number there
+  d.floor = __fmaf_ru(-680.0f, st.t, rs.m);
   d.scale = kExp2Entries * 1.4426950408889634074 / st.t;
   d.without = -1;
   d.mode = kDrawP;

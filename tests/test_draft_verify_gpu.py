@@ -366,3 +366,23 @@ def test_greedy_takes_the_first_of_several_infinities(dtype):
     d[1] = 2048
     accepted, tokens, _ = check(z, d, cu, u, r, temps=0.0)
     assert accepted.tolist() == [1, 1, 0] and tokens.tolist() == [5, 2047, -1, 7, 0, 3]
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("temp", [1e-6, 2e-6, 3e-5])
+@pytest.mark.parametrize("level", [1500.0, -1500.0, 10000.0, 70.0, 1e6])
+def test_low_temperatures_and_logits_a_few_steps_apart(level, temp, probs):
+    """The coldest temperatures that are not greedy, with logits of one size: neighbouring fp32 values are up to tens of
+    thousands of T apart, and the cutoff below which a weight is 0 falls between two of them."""
+    counts = [3, 0, 2, 1, 4]
+    step = float(np.spacing(np.float32(abs(level) * (1 - 2.0**-20))))
+    for v in (7, 500, 9001):
+        z, d, cu, u, r, q = make(counts, v, torch.float32, v)
+        g = torch.Generator(device=DEV).manual_seed(v)
+        z = level - step * torch.randint(0, 9, z.shape, device=DEV, generator=g).float()
+        z[1, :-1] -= 2 * step  # one token at the maximum
+        rows = torch.arange(len(d), device=DEV) + torch.repeat_interleave(torch.arange(5, device=DEV),
+                                                                          torch.tensor(counts, device=DEV))
+        d[::2] = z[rows].argmax(-1)[::2]
+        u[::3] = 0.0
+        check(z, d, cu, u, r, q if probs else None, temp)
