@@ -20,7 +20,9 @@
 //   sample  one cluster of 1 to 8 CTAs per sequence: merges the row statistics, decides a, then draws from
 //           the chosen row. Running sums and probabilities are in 64 bits: which token's interval a
 //           number falls in is a comparison over up to V borders, and sums in 32 bits would move each
-//           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256. It is
+//           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256. Acceptance is one
+//           comparison, which the statistics' fp32 sum decides unless the two sides are closer than that sum's
+//           error bound (stats_sum_error, 7e-5; one draft in some ten thousand): then the row is summed in 64 bits. It is
 //           bound by issue slots and the 64-bit pipe (64 lanes per SM and clock), so the exponential is a
 //           short one of its own (exp2_scaled below). 64 sequences of V = 128256 with draft probabilities: 55 us
 //           in all; per cluster 5 us for the decision, 7 for a pass over a row, 3 for the search.
@@ -198,6 +200,7 @@ struct VerifyArgs {
   int row_step;    // stats: rows of a sequence are dealt to this many blocks
   int early;       // stats: the sample kernel may start beside this one
   int strip_step;  // sample: 256-column strips per group of columns
+  double sum_error;  // relative error of a row's sum of the statistics
   Exp2Table exp2;
 };
 
@@ -397,6 +400,8 @@ __device__ __forceinline__ Decision ld_cluster_decision(const Decision* local, u
   return d;
 }
 
+constexpr int kPassOpen = 2;  // a draft whose acceptance the fp32 sum of its row cannot decide
+
 // What the next token is drawn from.
 enum DrawMode : int { kDrawP = 0, kDrawWithout = 1, kDrawResidual = 2 };
 
@@ -498,10 +503,54 @@ __device__ __forceinline__ double sum_columns(const VerifyArgs& a, const DrawRow
   return all;
 }
 
+// The part of a row's fp32 sum s of exp((z - m) / T) by which that sum may be off, with h = 2^-24: exponents
+// a = (z - m) k, each of 4 roundings, where |a| <= 55 (what lies below adds less than 2^30 2^-55): 4 * 55 ln 2 = 153 h; the
+// same again for the rises of the maximum, 4 h for ex2.approx, 10 h for a lane's sum of one load, 6 h for each of up to 64
+// loads and 6 h for each of 14 + n_chunks / 32 joins: below (800 + n_chunks) h.
+inline double stats_sum_error(int n_chunks) { return (1024.0 + n_chunks) / (1 << 24); }
+
+// Row `z` for draws and sums over all its tokens; m: its maximum.
+__device__ __forceinline__ DrawRow draw_row(const void* z, float m, float t) {
+  DrawRow d;
+  d.z = z;
+  d.q = nullptr;
+  d.m = m;
+  // rounded up: at 1500 and T = 1e-6 a step of fp32 is 122 T, and a cutoff rounded down would let in logits below the
+  // range of exp2_scaled, whose results are some number there
+  d.floor = __fmaf_ru(-680.0f, t, m);
+  d.scale = kExp2Entries * 1.4426950408889634074 / t;
+  d.without = -1;
+  d.mode = kDrawP;
+  return d;
+}
+
+// Sum of exp((z - m) / T) over a whole row in 64 bits, by all threads of the CTA (table: of scale 1). Out of line: one draft
+// in some ten thousand needs it.
+template <typename T>
+__device__ __noinline__ double row_sum_f64(const VerifyArgs& a, const void* z, float m, float t, const double* table,
+                                           double (*s_lane)[kVfyThreads], double* s_warp) {
+  const DrawRow d = draw_row(z, m, t);
+  constexpr int kSpan = 256 * kVfyWarps;
+  const int strips = static_cast<int>((a.vocab + kSpan - 1) / kSpan);
+  const int group_cols = 256 * ((strips + kVfyMaxGroups - 1) / kVfyMaxGroups);
+  const int64_t per_warp = ((a.vocab + kVfyWarps - 1) / kVfyWarps + group_cols - 1) / group_cols * group_cols;
+  const int warp = threadIdx.x >> 5;
+  const int lo = static_cast<int>(min(a.vocab, warp * per_warp));
+  const int hi = static_cast<int>(min(a.vocab, lo + per_warp));
+  const double mine = warp_sum(sum_columns<T, float, false>(a, d, table, lo, hi, group_cols, s_lane));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s_warp[warp] = mine;
+  __syncthreads();
+  double total = 0.0;
+  for (int w = 0; w < kVfyWarps; ++w) total += s_warp[w];
+  return total;
+}
+
 template <typename T, typename Q>
 __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ int s_pass[kVfyWarps];
   __shared__ double s_x[kVfyWarps];
+  __shared__ double s_uq[kVfyWarps];
   __shared__ Decision s_decision;
   __shared__ double s_warp[kVfyWarps];
   __shared__ double s_total[2];  // read by the other CTAs of the cluster; one per exchange
@@ -549,19 +598,34 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
         if (lane == 0) {
           const double x = (static_cast<double>(z) - r.m) / st.t;
           int pass = 0;
-          if (valid && r.s > 0.0f)
-            pass = st.greedy ? static_cast<uint32_t>(d) == r.idx : static_cast<double>(u) * qd * r.s < exp(x);
+          if (valid && r.s > 0.0f) {
+            if (st.greedy) {
+              pass = static_cast<uint32_t>(d) == r.idx;
+            } else {
+              const double uq = static_cast<double>(u) * qd, e = exp(x);
+              const double off = r.s * a.sum_error;
+              pass = uq * (r.s + off) < e ? 1 : (uq * (r.s - off) < e ? kPassOpen : 0);
+              s_uq[warp] = uq;
+            }
+          }
           s_pass[warp] = valid || i == n ? pass : -1;
           s_x[warp] = x;
           s_rows[warp] = r;
         }
       }
       __syncthreads();
-      for (int w = 0; w < kVfyWarps && i0 + w <= n; ++w)
-        if (s_pass[w] != 1) {
+      for (int w = 0; w < kVfyWarps && i0 + w <= n; ++w) {
+        int pass = s_pass[w];
+        if (pass == kPassOpen) {  // too close to the border for a sum in 32 bits
+          const double sum = row_sum_f64<T>(a, logits + (row0 + i0 + w) * a.ld_logits, s_rows[w].m, st.t, s_exp2, s_lane,
+                                            s_warp);
+          pass = s_uq[w] * sum < exp(s_x[w]);
+        }
+        if (pass != 1) {
           acc = i0 + w;
           break;
         }
+      }
       const int64_t upto = acc < 0 ? i0 + kVfyWarps : acc;
       if (threadIdx.x < kVfyWarps && i0 + threadIdx.x < upto) {
         a.tokens[row0 + i0 + threadIdx.x] = __ldg(a.drafts + lo + i0 + threadIdx.x);
@@ -603,16 +667,8 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
   }
 
   // ---- draw from row `row`
-  DrawRow d;
-  d.z = logits + row * a.ld_logits;
+  DrawRow d = draw_row(logits + row * a.ld_logits, rs.m, st.t);
   d.q = a.q == nullptr ? nullptr : static_cast<const Q*>(a.q) + (lo + acc) * a.ld_q;
-  d.m = rs.m;
-  // rounded up: at 1500 and T = 1e-6 a step of fp32 is 122 T, and a cutoff rounded down would let in logits below the
-  // range of exp2_scaled, whose results are some number there
-  d.floor = __fmaf_ru(-680.0f, st.t, rs.m);
-  d.scale = kExp2Entries * 1.4426950408889634074 / st.t;
-  d.without = -1;
-  d.mode = kDrawP;
   // columns of this CTA, and of each of its warps, in order, in groups of strip_step strips of 256
   const int group_cols = 256 * a.strip_step;
   const int warps = static_cast<int>(ctas) * kVfyWarps;
@@ -819,6 +875,7 @@ static int launch_verify(VerifyArgs& a, cudaStream_t stream) {
   while (a.chunk_cols < 16 * kVfyChunk && rows * ((a.vocab + 2 * a.chunk_cols - 1) / (2 * a.chunk_cols)) >= 32ll * sms)
     a.chunk_cols *= 2;
   a.n_chunks = static_cast<int>((a.vocab + 7 + a.chunk_cols - 1) / a.chunk_cols);
+  a.sum_error = stats_sum_error(a.n_chunks);
   const int64_t mean_rows = (a.n_drafts + 2 * a.batch - 1) / a.batch;
   a.row_step = static_cast<int>(mean_rows < 64 ? mean_rows : 64);
   const dim3 grid(static_cast<unsigned>((a.n_chunks + kVfyWarps - 1) / kVfyWarps),

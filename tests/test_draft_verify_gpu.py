@@ -386,3 +386,23 @@ def test_low_temperatures_and_logits_a_few_steps_apart(level, temp, probs):
         d[::2] = z[rows].argmax(-1)[::2]
         u[::3] = 0.0
         check(z, d, cu, u, r, q if probs else None, temp)
+
+
+@pytest.mark.parametrize("dtype,probs", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16),
+                                         (torch.float16, None), (torch.float32, None)])
+@pytest.mark.parametrize("v,b", [(3, 200), (2051, 300), (32000, 30), (128256, 8)])
+def test_acceptance_next_to_its_border(v, b, dtype, probs):
+    """Numbers a few fp32 steps (6e-8 to 1.2e-7 each) either side of p(d) / q(d). The border is known to 1e-11 (an exponential of
+    1.6e-12, sums of 64 bits), so numbers closer to it than that are moved by a step first."""
+    for drafts in (1, 3):
+        z, d, cu, u, r, q = make([drafts] * b, v, dtype, v + drafts, probs, spread=1.0)
+        rows = torch.arange(len(d), device=DEV) + torch.arange(len(d), device=DEV) // drafts
+        for temp in (1.0, 0.7):
+            p = torch.softmax(z[rows].double() / float(np.float32(temp)), -1).gather(1, d[:, None])[:, 0]
+            qd = torch.ones_like(p) if q is None else q.double().gather(1, d[:, None])[:, 0]
+            near = (p / qd).float()
+            for steps in (-2, -1, 0, 1, 2):
+                bits = near.view(torch.int32) + steps
+                x = bits.view(torch.float32)
+                x = torch.where((x.double() * qd / p - 1).abs() < 1e-11, (bits + 1).view(torch.float32), x)
+                check(z, d, cu, x, r, q, temp)
