@@ -496,10 +496,10 @@ struct Int8CEPartialsEpilogue {
       s2[i & 1] = add_f32x2(s2[i & 1], e);
       u2[i & 1] = fma_f32x2(dd, e, u2[i & 1]);
     }
-    // d * e0 first: columns behind a mask (or with logits of -1e37) leave a d whose product with s passes the
+    // s * e0 first: columns behind a mask (or with logits of -1e37) leave a d whose product with s passes the
     // largest float, and infinity times an e0 of 0 would be NaN
-    st.u = fmaf(d * e0, st.s, st.u * e0);
     st.s *= e0;
+    st.u = fmaf(d, st.s, st.u * e0);
     st.m = top;
     float f0, f1;
     unpack_f32x2(add_f32x2(s2[0], s2[1]), f0, f1);
@@ -573,8 +573,9 @@ struct Int8CEPartialsEpilogue {
       const float top = fmaxf(st.m, o.x);
       const float d0 = st.m - top, d1 = o.x - top;
       const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
-      st.u = fmaf(d0 * e0, st.s, st.u * e0) + fmaf(d1 * e1, o.y, o.z * e1);  // as in columns16
-      st.s = st.s * e0 + o.y * e1;
+      const float s0 = st.s * e0, s1 = o.y * e1;
+      st.u = fmaf(d0, s0, st.u * e0) + fmaf(d1, s1, o.z * e1);  // as in columns16
+      st.s = s0 + s1;
       st.m = top;
     }
     if (row_ok && device_check(n_blk < p.n_tiles, p.status))
@@ -756,8 +757,9 @@ struct FewScore {
           const float top = fmaxf(t.x, o.x);
           const float d0 = t.x - top, d1 = o.x - top;
           const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
-          t.z = fmaf(d0 * e0, t.y, t.z * e0) + fmaf(d1 * e1, o.y, o.z * e1);  // d * e first: no overflow
-          t.y = t.y * e0 + o.y * e1;
+          const float s0 = t.y * e0, s1 = o.y * e1;
+          t.z = fmaf(d0, s0, t.z * e0) + fmaf(d1, s1, o.z * e1);  // as in columns16
+          t.y = s0 + s1;
           t.x = top;
         }
         if (token < rows && w.tile * 128 < p.op.cols && device_check(w.tile < p.n_tiles, status))
