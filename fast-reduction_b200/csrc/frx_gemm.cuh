@@ -337,8 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
   uint64_t* acc_full = empty + Cfg::kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* mma_done = acc_empty + 2;
-  uint64_t* join = mma_done + 1;  // kI8: one per pair of epilogue warps that share their rows
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(join + (kI8 ? 8 : 0));
+  uint64_t* join = mma_done + 1;  // kI8: two per pair of epilogue warps that share their rows, one each way
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(join + (kI8 ? 16 : 0));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // uniform over the grid (both CTAs of every pair), so an early return skips every barrier together
   if (!device_check(reinterpret_cast<const uint8_t*>(tmem_slot + 2) - smem_raw <=
@@ -363,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
       mbar_init(&acc_empty[b], kI8 ? 16 : 8);  // one arrival per epilogue warp of both CTAs
     }
     mbar_init(mma_done, 1);
-    for (int j = 0; j < (kI8 ? 8 : 0); ++j) mbar_init(&join[j], 1);
+    for (int j = 0; j < (kI8 ? 16 : 0); ++j) mbar_init(&join[j], 1);
     *abort_flag = 0;
     fence_mbarrier_init();
   }
@@ -524,7 +524,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
     constexpr int kGroups = kI8 ? 2 : 1;  // each takes every second tile, from its own accumulator
     const int group = kI8 ? ((warp - 2) >> 2) & 1 : 0;
     const int half = kI8 ? (warp - 2) >> 3 : 0;  // which 128 columns of a tile
-    uint32_t joins = 0;  // parity of this warp pair's next join
+    uint32_t joins = 0;  // joins of this warp pair so far
     [[maybe_unused]] typename EpiTile<Epi, kI8>::type tile{}, next{};
     if constexpr (kI8) {
       if (pair_id + group * num_pairs < sched.num_tiles) {
@@ -569,13 +569,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8 ? kGemmThreadsI8
       };
       if constexpr (kI8) {
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-          int done = 1;
-          if (lane == 0)
-            done = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, sched.wait_limit_ns);
-          return __shfl_sync(0xffffffffu, done, 0) != 0;
+          // by every lane, since what the barrier hands over is every lane's to read
+          const bool done =
+              mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue, sched.wait_limit_ns);
+          return __all_sync(0xffffffffu, done) != 0;
         };
         if (!Epi::run(ep, tile, s_epi, tacc + static_cast<uint32_t>(half * 128), pm * 2 + static_cast<int>(rank), pn,
-                      group, half, q, lane, &join[group * 4 + q], joins, release, wait))
+                      group, half, q, lane, &join[2 * (group * 4 + q)], joins, release, wait))
           break;
         tile = next;
       } else {

@@ -374,7 +374,7 @@ __device__ __forceinline__ float4 nothing_live(float s, float zt) {
 //   kFull = true: z = (acc * wscale) * xs + bias, for a bias and for the caller's own scales (any sign).
 template <bool kFull>
 struct Int8CEPartialsEpilogue {
-  static constexpr int kJoinBytes = 8 * 32 * 16;  // (group, quarter) x 32 tokens
+  static constexpr int kJoinBytes = 2 * 8 * 32 * 16;  // (receiving half, group, quarter) x 32 tokens
   static constexpr int kSmemBytes = kJoinBytes + 16 * 1024;  // and 128 scales and 128 biases per warp
 
   struct Params {
@@ -551,25 +551,27 @@ struct Int8CEPartialsEpilogue {
     st.m *= f;
     st.u *= f;
     st.zt *= f;
-    // The second half hands over through shared memory. The first gives the accumulator back only after it
-    // has read the slot, so the second cannot be at its next tile's write by then.
-    float4* slot = reinterpret_cast<float4*>(smem) + (group * 4 + q) * 32 + lane;
-    if (half == 1) {
+    // One half hands its statistics to the other through shared memory, in turn: the first half receives the pair's first
+    // tile's, the second half the next one's. A half that writes its slot has then received since the other read it (its
+    // own wait on the other's arrival, which follows that read), so no write passes a read.
+    const int turn = static_cast<int>(joins & 1u);
+    const uint32_t parity = (joins >> 1) & 1u;
+    ++joins;
+    float4* slot = reinterpret_cast<float4*>(smem) + ((turn * 2 + group) * 4 + q) * 32 + lane;
+    if (half != turn) {
       *slot = make_float4(st.m, st.s, st.u, st.zt);
       __syncwarp();
-      if (lane == 0) mbar_arrive(join);
+      if (lane == 0) mbar_arrive(join + turn);
       release();
       return true;
     }
-    const bool joined = wait(join, joins);
-    joins ^= 1u;
-    if (!joined) return false;
+    if (!wait(join + turn, parity)) return false;
     const float4 o = *slot;
     release();
     st.zt += o.w;
-    if (st.s == 0.0f) {  // nothing in the first half
+    if (st.s == 0.0f) {  // nothing in this half
       st = {o.x, o.y, o.z, st.zt};
-    } else if (o.y != 0.0f) {  // something in the second one, which the tile need not reach
+    } else if (o.y != 0.0f) {  // something in the other one (the tile need not reach the second)
       const float top = fmaxf(st.m, o.x);
       const float d0 = st.m - top, d1 = o.x - top;
       const float e0 = ex2_approx(d0 * kLog2e), e1 = ex2_approx(d1 * kLog2e);
@@ -932,6 +934,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         good = mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue);
       return __shfl_sync(0xffffffffu, good, 0) != 0;
     };
+    auto join_wait = [&](uint64_t* bar, uint32_t parity) {
+      // by every lane, since what the barrier hands over is every lane's to read
+      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, status, kStatusTimeoutEpilogue)) != 0;
+    };
     for (int i = 0; i < my_tiles; ++i) {
       w.buf = i & 1;
       const uint32_t parity = static_cast<uint32_t>((i >> 1) & 1);
@@ -947,7 +953,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[w.buf]);
       };
-      if (!Epi::run(ep, w, s_epi, join, parity, status, release, wait)) break;
+      if (!Epi::run(ep, w, s_epi, join, parity, status, release, join_wait)) break;
     }
   }
   tc_fence_before();

@@ -448,3 +448,23 @@ def test_masked_stretch_before_live_columns(rows, codes, fill):
         assert ((ce.double() - ce_r).abs() <= tol_ce).all(), stretch
         assert ((ent.double() - ent_r).abs() <= tol_ent).all(), stretch
         assert torch.equal(lp, -ce)
+
+
+@pytest.mark.parametrize("rows,k", [(129, 16), (300, 64), (700, 200)])
+def test_score_of_many_tiles_per_cta(rows, k):
+    """Short sums and a long vocabulary: the epilogue's two halves hand over through the same slots up to 20 times a CTA,
+    with nothing else to wait for."""
+    from fast_reduction import int8_ce_entropy
+
+    v = 128256
+    x, w, ws, b = make(rows, k, v, torch.bfloat16, rows, torch.float32)
+    t = torch.randint(0, v, (rows,), device=DEV, generator=_gen(4))
+    for bias in (None, b):
+        c, s = ref_quantize(x)
+        ce_r, ent_r, tol_ce, tol_ent = ref_score(*ref_logits(c, s, w, ws, bias), t)
+        first = int8_ce_entropy(x, w, ws, t, bias=bias)
+        assert ((first[0].double() - ce_r).abs() <= tol_ce).all()
+        assert ((first[1].double() - ent_r).abs() <= tol_ent).all()
+        for _ in range(20):
+            for a, e in zip(int8_ce_entropy(x, w, ws, t, bias=bias), first):
+                assert torch.equal(a, e)
