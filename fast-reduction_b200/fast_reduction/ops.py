@@ -515,6 +515,12 @@ def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
     return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 
 
+def _leading(t: torch.Tensor) -> int:
+    """Row stride of a matrix for the C entry points: one row may come with any (torch calls that contiguous)."""
+    rows, cols = t.shape
+    return max(t.stride(0), cols) if rows <= 1 else t.stride(0)
+
+
 def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
     """codes (int8), scale (fp32 per row) <- symmetric 8-bit codes of the rows of x (frx_quantize_i8)."""
     dev = _require_cuda(x, codes, scale)
@@ -522,10 +528,13 @@ def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> No
         raise TypeError("quantize_i8 takes a bfloat16, float16 or float32 matrix, int8 codes and float32 scales")
     if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
         raise ValueError("codes must have x's shape and scale one value per row")
+    rows, cols = x.shape
+    if cols > 1 and (x.stride(1) != 1 or codes.stride(1) != 1):
+        raise ValueError("x and codes must have unit column stride")
     lib = nat.load()
     with torch.cuda.device(dev):
         rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
-            x.data_ptr(), _OUT_DTYPES[x.dtype], x.stride(0), x.shape[0], x.shape[1], codes.data_ptr(), codes.stride(0),
+            x.data_ptr(), _OUT_DTYPES[x.dtype], _leading(x), rows, cols, codes.data_ptr(), _leading(codes),
             scale.data_ptr(), nat.stream_of(dev)))
     nat.check(rc, "frx_quantize_i8")
 
@@ -547,7 +556,7 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias):
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
     ldx, unit = x.stride()
     ldw, wunit = weight.stride()
-    if unit != 1 or wunit != 1:
+    if (unit != 1 or wunit != 1) and k > 1:
         raise ValueError("x and weight must have unit column stride")
     if not _is_vector(weight_scale, torch.float32, cols):
         raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
@@ -609,14 +618,14 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
     dt = _LOGITS_DTYPES.get(logits.dtype)
     rows, vocab = logits.shape
     ldl, unit = logits.stride()
-    if dt is None or rows != n + batch or unit != 1:
+    if dt is None or rows != n + batch or (unit != 1 and vocab > 1):
         raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V] with unit column stride, got "
                          f"{logits.dtype} {tuple(logits.shape)} stride {logits.stride()}")
     qptr, qdt, ldq = None, 0, 0
     if draft_probs is not None:
         qdt = _LOGITS_DTYPES.get(draft_probs.dtype)
         ldq, unit = draft_probs.stride()
-        if qdt is None or draft_probs.shape != (n, vocab) or unit != 1:
+        if qdt is None or draft_probs.shape != (n, vocab) or (unit != 1 and vocab > 1):
             raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}] with unit column stride, "
                              f"got {draft_probs.dtype} {tuple(draft_probs.shape)} stride {draft_probs.stride()}")
         qptr = draft_probs.data_ptr()

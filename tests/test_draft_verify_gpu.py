@@ -406,3 +406,19 @@ def test_acceptance_next_to_its_border(v, b, dtype, probs):
                 x = bits.view(torch.float32)
                 x = torch.where((x.double() * qd / p - 1).abs() < 1e-11, (bits + 1).view(torch.float32), x)
                 check(z, d, cu, x, r, q, temp)
+
+
+def test_strides_of_dimensions_of_one():
+    """One row, or one token, whose stride torch does not care for."""
+    from fast_reduction import verify_drafts
+
+    e, ids = torch.empty(0, device=DEV), torch.empty(0, device=DEV, dtype=torch.int64)
+    row = torch.randn(90, 1, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    z = row.t()
+    assert z.shape == (1, 90) and z.stride(0) != 90
+    check(z, ids, torch.tensor([0, 0], device=DEV), e, torch.tensor([0.4], device=DEV))
+    z, d, cu, u, r, q = make([2, 1], 1, torch.float32, 3)
+    flat_z, flat_q = z.reshape(1, 5).t(), q.reshape(1, 3).t()
+    assert flat_z.stride(1) == 5 and flat_q.stride(1) == 3
+    got, want = verify_drafts(flat_z, d, cu, u, r, flat_q), verify_drafts(z, d, cu, u, r, q)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

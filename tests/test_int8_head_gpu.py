@@ -468,3 +468,33 @@ def test_score_of_many_tiles_per_cta(rows, k):
         for _ in range(20):
             for a, e in zip(int8_ce_entropy(x, w, ws, t, bias=bias), first):
                 assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_strides_of_dimensions_of_one(dtype):
+    """One row, or one column, whose stride torch does not care for: a transposed column, a row of an expanded matrix, a
+    column of a transposed row."""
+    from fast_reduction import int8_ce_entropy, int8_linear, quantize_int8
+
+    k = 70
+    col = torch.randn(k, 1, device=DEV, generator=_gen(1)).to(dtype)
+    wide = torch.randn(1, k, device=DEV, generator=_gen(2)).to(dtype)
+    w, ws = quantize_int8(torch.randn(300, k, device=DEV, generator=_gen(3)))
+    t = torch.tensor([7], device=DEV)
+    for x in (col.t(), wide.expand(5, k)[:1], wide.expand(5, k)[2:3], wide.as_strided((1, k), (3, 1))):
+        assert x.shape == (1, k) and x.stride(0) != k
+        c, s = ref_quantize(x)
+        codes, scale = quantize_int8(x)
+        assert torch.equal(codes.double(), c) and torch.equal(scale, s)
+        assert_logits(int8_linear(x, w, ws), *ref_logits(c, s, w, ws, None))
+        for a, e in zip(int8_ce_entropy(x, w, ws, t), int8_ce_entropy(x.clone().view(1, k), w, ws, t)):
+            assert torch.equal(a, e)
+    one = torch.randn(1, 40, device=DEV, generator=_gen(4)).to(dtype)
+    w1, ws1 = quantize_int8(torch.randn(300, 1, device=DEV, generator=_gen(5)))
+    for x in (one.t(), one.t()[:1]):
+        assert x.shape[1] == 1 and x.stride(1) == 40
+        c, s = ref_quantize(x)
+        codes, scale = quantize_int8(x)
+        assert torch.equal(codes.double(), c) and torch.equal(scale, s)
+        assert_logits(int8_linear(x, w1, ws1), *ref_logits(c, s, w1, ws1, None))
+        assert torch.equal(int8_linear(codes, w1, ws1, hidden_scale=scale, out_dtype=dtype), int8_linear(x, w1, ws1))
