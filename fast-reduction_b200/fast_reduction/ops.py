@@ -515,10 +515,24 @@ def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
     return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 
 
-def _leading(t: torch.Tensor) -> int:
-    """Row stride of a matrix for the C entry points: one row may come with any (torch calls that contiguous)."""
+def _leading(t: torch.Tensor, name: str) -> int:
+    """Row stride of a matrix for the C entry points. A dimension of one may come with any stride (torch calls that
+    contiguous); otherwise columns lie next to each other and rows do not overlap."""
     rows, cols = t.shape
-    return max(t.stride(0), cols) if rows <= 1 else t.stride(0)
+    ld, unit = t.stride()
+    if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
+        raise ValueError(f"{name} must have unit column stride and rows that do not overlap, got shape {tuple(t.shape)} "
+                         f"stride {t.stride()}")
+    return ld if ld > cols else cols
+
+
+def _room(workspace: torch.Tensor | None, dtype: torch.dtype) -> tuple[int | None, int]:
+    """Address and number of elements of a workspace."""
+    if workspace is None:
+        return None, 0
+    if workspace.dtype is not dtype or not workspace.is_contiguous():
+        raise ValueError(f"the workspace must be contiguous {dtype}, got {workspace.dtype} stride {workspace.stride()}")
+    return workspace.data_ptr(), workspace.numel()
 
 
 def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> None:
@@ -529,13 +543,12 @@ def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> No
     if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
         raise ValueError("codes must have x's shape and scale one value per row")
     rows, cols = x.shape
-    if cols > 1 and (x.stride(1) != 1 or codes.stride(1) != 1):
-        raise ValueError("x and codes must have unit column stride")
+    ldx, ldc = _leading(x, "x"), _leading(codes, "codes")
     lib = nat.load()
     with torch.cuda.device(dev):
         rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
-            x.data_ptr(), _OUT_DTYPES[x.dtype], _leading(x), rows, cols, codes.data_ptr(), _leading(codes),
-            scale.data_ptr(), nat.stream_of(dev)))
+            x.data_ptr(), _OUT_DTYPES[x.dtype], ldx, rows, cols, codes.data_ptr(), ldc, scale.data_ptr(),
+            nat.stream_of(dev)))
     nat.check(rc, "frx_quantize_i8")
 
 
@@ -545,8 +558,9 @@ def i8_workspace_bytes(x: torch.Tensor) -> int:
     return 0 if x.dtype == torch.int8 else (rows * ((k + 15) // 16 * 16 + 4) + 15) // 16 * 16
 
 
-def _i8_operands(x, x_scale, weight, weight_scale, bias):
-    """Checked operands of an 8-bit product: (device, rows, cols, k, the leading C arguments up to bias_dtype)."""
+def _i8_operands(x, x_scale, weight, weight_scale, bias, *others):
+    """Checked operands of an 8-bit product: (device, rows, cols, k, the leading C arguments up to bias_dtype). ``others``
+    need to be on the same device."""
     xdt = _I8_X_DTYPES.get(x.dtype)
     if xdt is None or weight.dtype is not torch.int8:
         raise TypeError(f"x must be int8, bfloat16, float16 or float32 and weight int8, got {x.dtype} and {weight.dtype}")
@@ -554,10 +568,7 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias):
     cols, wk = weight.shape
     if wk != k:
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
-    ldx, unit = x.stride()
-    ldw, wunit = weight.stride()
-    if (unit != 1 or wunit != 1) and k > 1:
-        raise ValueError("x and weight must have unit column stride")
+    ldx, ldw = _leading(x, "x"), _leading(weight, "weight")
     if not _is_vector(weight_scale, torch.float32, cols):
         raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
                          f"{tuple(weight_scale.shape)}")
@@ -576,21 +587,20 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias):
             raise ValueError(f"bias must be a contiguous bfloat16, float16 or float32 [{cols}], got {bias.dtype} "
                              f"{tuple(bias.shape)}")
         bptr = bias.data_ptr()
-    dev = _one_device(x, x_scale, weight, weight_scale, bias)
-    return dev, rows, cols, k, (x.data_ptr(), xdt, max(ldx, k), sptr, weight.data_ptr(), max(ldw, k),
-                                weight_scale.data_ptr(), bptr, bdt)
+    dev = _one_device(x, x_scale, weight, weight_scale, bias, *others)
+    return dev, rows, cols, k, (x.data_ptr(), xdt, ldx, sptr, weight.data_ptr(), ldw, weight_scale.data_ptr(), bptr, bdt)
 
 
 def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
             out: torch.Tensor, workspace: torch.Tensor | None, *, bias: torch.Tensor | None = None) -> None:
     """out[r, j] <- (xc[r] . weight[j]) * x_scale[r] * weight_scale[j] (+ bias[j]): xc = x for int8 x, else its codes,
     which go into the uint8 ``workspace`` (frx_gemm_i8)."""
-    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
+    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias, out, workspace)
     odt = _OUT_DTYPES.get(out.dtype)
-    if odt is None or out.shape != (rows, cols) or out.device != dev:
-        raise ValueError(f"out must be bfloat16, float16 or float32 [{rows}, {cols}] on {dev}")
-    _call("gemm_i8", "frx_gemm_i8", dev, *operands, rows, cols, k, None if workspace is None else workspace.data_ptr(),
-          0 if workspace is None else workspace.numel(), out.data_ptr(), max(out.stride(0), cols), odt)
+    if odt is None or out.shape != (rows, cols):
+        raise ValueError(f"out must be bfloat16, float16 or float32 [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
+    _call("gemm_i8", "frx_gemm_i8", dev, *operands, rows, cols, k, *_room(workspace, torch.uint8), out.data_ptr(),
+          _leading(out, "out"), odt)
 
 
 def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -598,15 +608,15 @@ def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.T
                   workspace: torch.Tensor, *, launch_rows: int, ignore_index: int,
                   bias: torch.Tensor | None = None) -> None:
     """ce, entropy, log_probs <- those of gemm_i8's fp32 logits, launch_rows rows at a time (frx_i8_ce_entropy)."""
-    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias)
-    if target.dtype != torch.int64 or not target.is_contiguous() or target.numel() != rows or target.device != dev:
-        raise ValueError("target must be a contiguous int64 tensor with one id per row, on the tokens' device")
+    dev, rows, cols, k, operands = _i8_operands(x, x_scale, weight, weight_scale, bias, target, ce, entropy, log_probs,
+                                                workspace)
+    if target.dtype != torch.int64 or not target.is_contiguous() or target.numel() != rows:
+        raise ValueError("target must be a contiguous int64 tensor with one id per row")
     for t in (ce, entropy, log_probs):
         if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != rows:
             raise ValueError("ce, entropy and log_probs must be contiguous float32 with one value per row")
     _call("i8_ce_entropy", "frx_i8_ce_entropy", dev, *operands, target.data_ptr(), rows, cols, k, ignore_index,
-          launch_rows, workspace.data_ptr(), workspace.numel(), ce.data_ptr(), entropy.data_ptr(), None,
-          log_probs.data_ptr())
+          launch_rows, *_room(workspace, torch.uint8), ce.data_ptr(), entropy.data_ptr(), None, log_probs.data_ptr())
 
 
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor, uniforms: torch.Tensor,
@@ -617,18 +627,17 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
     n, batch = drafts.numel(), cu_drafts.numel() - 1
     dt = _LOGITS_DTYPES.get(logits.dtype)
     rows, vocab = logits.shape
-    ldl, unit = logits.stride()
-    if dt is None or rows != n + batch or (unit != 1 and vocab > 1):
-        raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V] with unit column stride, got "
-                         f"{logits.dtype} {tuple(logits.shape)} stride {logits.stride()}")
+    if dt is None or rows != n + batch:
+        raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V], got {logits.dtype} "
+                         f"{tuple(logits.shape)}")
+    ldl = _leading(logits, "logits")
     qptr, qdt, ldq = None, 0, 0
     if draft_probs is not None:
         qdt = _LOGITS_DTYPES.get(draft_probs.dtype)
-        ldq, unit = draft_probs.stride()
-        if qdt is None or draft_probs.shape != (n, vocab) or (unit != 1 and vocab > 1):
-            raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}] with unit column stride, "
-                             f"got {draft_probs.dtype} {tuple(draft_probs.shape)} stride {draft_probs.stride()}")
-        qptr = draft_probs.data_ptr()
+        if qdt is None or draft_probs.shape != (n, vocab):
+            raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}], got {draft_probs.dtype} "
+                             f"{tuple(draft_probs.shape)}")
+        qptr, ldq = draft_probs.data_ptr(), _leading(draft_probs, "draft_probs")
     if not _is_vector(drafts, torch.int64, n) or not _is_vector(cu_drafts, torch.int64, batch + 1):
         raise ValueError("drafts and cu_drafts must be contiguous int64 vectors")
     if not _is_vector(uniforms, torch.float32, n):
@@ -646,8 +655,8 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
             and _is_vector(log_probs, torch.float32, rows)):
         raise ValueError(f"outputs must be contiguous: int64 accepted [{batch}], int64 tokens and float32 log_probs "
                          f"[{rows}]")
-    dev = _one_device(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature)
-    _call("verify_drafts", "frx_verify_drafts", dev, logits.data_ptr(), dt, max(ldl, vocab),
-          drafts.data_ptr(), cu_drafts.data_ptr(), uniforms.data_ptr(), final_uniforms.data_ptr(), qptr, qdt, max(ldq, vocab), tptr,
-          temperature_all, batch, n, vocab, workspace.data_ptr(), workspace.numel(), accepted.data_ptr(),
-          tokens.data_ptr(), log_probs.data_ptr())
+    dev = _one_device(logits, drafts, cu_drafts, uniforms, final_uniforms, draft_probs, temperature, workspace, accepted,
+                      tokens, log_probs)
+    _call("verify_drafts", "frx_verify_drafts", dev, logits.data_ptr(), dt, ldl, drafts.data_ptr(), cu_drafts.data_ptr(),
+          uniforms.data_ptr(), final_uniforms.data_ptr(), qptr, qdt, ldq, tptr, temperature_all, batch, n, vocab,
+          *_room(workspace, torch.float32), accepted.data_ptr(), tokens.data_ptr(), log_probs.data_ptr())

@@ -422,3 +422,20 @@ def test_strides_of_dimensions_of_one():
     assert flat_z.stride(1) == 5 and flat_q.stride(1) == 3
     got, want = verify_drafts(flat_z, d, cu, u, r, flat_q), verify_drafts(z, d, cu, u, r, q)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tensor_level_call_refuses_tensors_of_the_host():
+    from fast_reduction import ops
+
+    z, d, cu, u, r, q = make([2, 1], 50, torch.float32, 3)
+    ids = [torch.empty(n, device=DEV, dtype=torch.int64) for n in (2, 5)]
+    good = [z, d, cu, u, r, q, torch.ones(2, device=DEV), 1.0, torch.empty(20, device=DEV), *ids,
+            torch.empty(5, device=DEV)]
+    ops.verify_drafts(*good)
+    for i in (0, 1, 2, 3, 4, 5, 6, 8, 9, 10, 11):
+        args = list(good)
+        args[i] = args[i].cpu()
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.verify_drafts(*args)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.verify_drafts(*good[:8], torch.empty(1, device=DEV).expand(20), *good[9:])

@@ -498,3 +498,29 @@ def test_strides_of_dimensions_of_one(dtype):
         assert torch.equal(codes.double(), c) and torch.equal(scale, s)
         assert_logits(int8_linear(x, w1, ws1), *ref_logits(c, s, w1, ws1, None))
         assert torch.equal(int8_linear(codes, w1, ws1, hidden_scale=scale, out_dtype=dtype), int8_linear(x, w1, ws1))
+
+
+def test_tensor_level_calls_refuse_tensors_of_the_host():
+    """Every tensor of a call has to be on the GPU, outputs and workspaces too."""
+    from fast_reduction import ops
+
+    x, w, ws, b = make(4, 64, 100, torch.bfloat16, 1, torch.float32)
+    t = torch.zeros(4, device=DEV, dtype=torch.int64)
+    out, work = torch.empty(4, 100, device=DEV), torch.empty(1 << 16, device=DEV, dtype=torch.uint8)
+    r = [torch.empty(4, device=DEV) for _ in range(3)]
+    good = [x, None, w, ws, out, work]
+    for i in (0, 2, 3, 4, 5):
+        args = list(good)
+        args[i] = args[i].cpu()
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.gemm_i8(*args, bias=b)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.gemm_i8(x, None, w, ws, torch.empty(1, 100, device=DEV).expand(4, 100), work)
+    good = [x, None, w, ws, t, *r, work]
+    for i in (0, 2, 3, 4, 5, 6, 7, 8):
+        args = list(good)
+        args[i] = args[i].cpu()
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.i8_ce_entropy(*args, launch_rows=4, ignore_index=-100)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.gemm_i8(x, None, w, ws, out, work[:1].expand(1 << 16))

@@ -163,3 +163,52 @@ def test_verify_refusals():
         call(draft_probs=q[:, :19])
     with pytest.raises(ValueError, match="temperature"):
         call(temperature=torch.ones(3))
+
+
+def test_tensor_level_calls_refuse_layouts_that_pass_their_memory():
+    """Rows that overlap, spread columns and spread workspaces, which the C entry points cannot see."""
+    from fast_reduction import ops
+
+    x, w, s = torch.zeros(4, 32), torch.zeros(10, 32, dtype=torch.int8), torch.ones(10)
+    t, out, work = torch.zeros(4, dtype=torch.int64), torch.zeros(4, 10), torch.zeros(4096, dtype=torch.uint8)
+    r = [torch.zeros(4) for _ in range(3)]
+
+    def score(x, w, work):
+        ops.i8_ce_entropy(x, None, w, s, t, *r, work, launch_rows=4, ignore_index=-100)
+
+    def spread(rows, dtype):
+        return [m.to(dtype).as_strided(*at) for m, at in ((torch.zeros(1, 32), ((rows, 32), (0, 1))),
+                                                          (torch.zeros(32, rows), ((rows, 32), (1, rows))),
+                                                          (torch.zeros(rows, 64), ((rows, 32), (64, 2))))]
+
+    for bad in spread(4, torch.float32):
+        for fn in (lambda: ops.gemm_i8(bad, None, w, s, out, work), lambda: score(bad, w, work)):
+            with pytest.raises(ValueError, match="x must have unit"):
+                fn()
+    for bad in spread(10, torch.int8):
+        for fn in (lambda: ops.gemm_i8(x, None, bad, s, out, work), lambda: score(x, bad, work)):
+            with pytest.raises(ValueError, match="weight must have unit"):
+                fn()
+    for fn in (lambda: ops.gemm_i8(x, None, w, s, out, work), lambda: score(x, w, work)):
+        with pytest.raises(ValueError, match="CUDA"):
+            fn()
+    for bad in (torch.zeros(1, dtype=torch.uint8).expand(4096), work.view(torch.float32)):
+        with pytest.raises(ValueError, match="workspace"):
+            ops._room(bad, torch.uint8)
+    for bad in (torch.zeros(1, 10).expand(4, 10), torch.zeros(10, 4).t()):
+        with pytest.raises(ValueError, match="out must"):
+            ops._leading(bad, "out")
+    z, q, d = torch.zeros(5, 20), torch.full((3, 20), 0.05), torch.zeros(3, dtype=torch.int64)
+    cu, u, f, e = torch.tensor([0, 1, 3]), torch.zeros(3), torch.zeros(2), torch.zeros(20)
+
+    def verify(z, q):
+        ops.verify_drafts(z, d, cu, u, f, q, None, 1.0, e, torch.zeros(2, dtype=torch.int64),
+                          torch.zeros(5, dtype=torch.int64), torch.zeros(5))
+
+    with pytest.raises(ValueError, match="CUDA"):
+        verify(z, q)
+    for bad in (z[:1].expand(5, 20), torch.zeros(20, 5).t()):
+        with pytest.raises(ValueError, match="logits must have unit"):
+            verify(bad, q)
+    with pytest.raises(ValueError, match="draft_probs must have unit"):
+        verify(z, q[:1].expand(3, 20))
