@@ -12,6 +12,7 @@ import contextlib
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -505,10 +506,16 @@ def _one_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device
 
 
 def refuse_grad(what: str, *tensors: torch.Tensor | None) -> None:
-    """Raises where a result without a gradient would silently end the graph of one of the inputs."""
+    """Raises where a result without a gradient, or without a tangent, would silently end what one of the inputs takes
+    part in: reverse mode (unless gradients are disabled) or forward mode (which torch.no_grad() leaves on)."""
+    duals = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+        if duals and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no gradient in forward mode either: call it on the primal")
 
 
 def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:

@@ -212,3 +212,36 @@ def test_tensor_level_calls_refuse_layouts_that_pass_their_memory():
             verify(bad, q)
     with pytest.raises(ValueError, match="draft_probs must have unit"):
         verify(z, q[:1].expand(3, 20))
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent that would be dropped silently: in a dual tensor (also under no_grad, which leaves forward mode on) and in
+    jvp. Inputs without one pass on to the next check."""
+    from torch.autograd import forward_ad
+
+    from fast_reduction import int8_ce_entropy, int8_linear, quantize_int8, verify_drafts
+
+    x, w, s, b = torch.zeros(4, 32), torch.zeros(10, 32, dtype=torch.int8), torch.ones(10), torch.zeros(10)
+    t = torch.zeros(4, dtype=torch.int64)
+    z, q = torch.zeros(5, 20), torch.full((3, 20), 0.05)
+    rest = (torch.zeros(3, dtype=torch.int64), torch.tensor([0, 1, 3]), torch.zeros(3), torch.zeros(2))
+    calls = [(quantize_int8, x), (lambda h: int8_linear(h, w, s), x), (lambda v: int8_linear(x, w, v), s),
+             (lambda v: int8_linear(x, w, s, bias=v), b), (lambda o: int8_linear(x, w, s, out=o), torch.zeros(4, 10)),
+             (lambda v: int8_linear(x.to(torch.int8), w, s, hidden_scale=v), torch.ones(4)),
+             (lambda h: int8_ce_entropy(h, w, s, t), x), (lambda v: int8_ce_entropy(x, w, s, t, bias=v), b),
+             (lambda v: verify_drafts(v, *rest, q), z), (lambda v: verify_drafts(z, *rest, v), q)]
+    for fn, v in calls:
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            torch.func.jvp(fn, (v,), (torch.ones_like(v),))
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(v, torch.ones_like(v))
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                fn(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                fn(dual)
+            with pytest.raises(ValueError, match="CUDA"):
+                fn(v)
+            with pytest.raises(ValueError, match="CUDA"):
+                fn(forward_ad.unpack_dual(dual).primal)
+        with pytest.raises(ValueError, match="CUDA"):
+            fn(dual)
