@@ -167,7 +167,8 @@ def int8_ce_entropy(
     target = target.contiguous()
     chunk = gk._chunk_rows(chunk_size, B)
     dev = x.device
-    ce, ent, logp = torch.empty(3, B, device=dev, dtype=torch.float32).unbind(0)
+    # three tensors: views of one would share a version counter, and each would keep the memory of all
+    ce, ent, logp = (torch.empty(B, device=dev, dtype=torch.float32) for _ in range(3))
     if B:
         V = w.shape[0]
         if B <= nat.FRX_I8_FEW_ROWS:

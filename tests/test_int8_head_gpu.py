@@ -524,3 +524,22 @@ def test_tensor_level_calls_refuse_tensors_of_the_host():
             ops.i8_ce_entropy(*args, launch_rows=4, ignore_index=-100)
     with pytest.raises(ValueError, match="workspace"):
         ops.gemm_i8(x, None, w, ws, out, work[:1].expand(1 << 16))
+
+
+@pytest.mark.parametrize("rows", [6, 200])
+def test_results_of_scoring_are_tensors_of_their_own(rows):
+    """Each result can be changed in place while another is saved for a backward pass, and keeps no memory but its own."""
+    from fast_reduction import int8_ce_entropy
+
+    x, w, ws, _ = make(rows, 64, 300, torch.bfloat16, 2)
+    t = torch.zeros(rows, device=DEV, dtype=torch.int64)
+    for hidden, shape in ((x, (rows,)), (x.view(2, rows // 2, 64), (2, rows // 2))):
+        out = int8_ce_entropy(hidden, w, ws, t)
+        assert len({o.untyped_storage().data_ptr() for o in out}) == 3
+        assert all(o.shape == shape and o.untyped_storage().nbytes() == 4 * rows for o in out)
+        a = torch.ones(shape, device=DEV, requires_grad=True)
+        loss = (a * out[1]).sum()  # saves the entropy
+        out[0].mul_(2)
+        out[2].zero_()
+        loss.backward()
+        assert torch.equal(a.grad, out[1])
