@@ -1182,6 +1182,10 @@ extern "C" int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t l
   const int64_t n_tiles = vocab_size > 0 ? (vocab_size + tile - 1) / tile : 0;
   const int64_t step = few || launch_rows >= rows ? rows : launch_rows;
   FRX_CHECK_RANGE(target, rows * 8, "frx_i8_ce_entropy: target");
+  FRX_CHECK_RANGE(ce, rows * 4, "frx_i8_ce_entropy: ce");
+  FRX_CHECK_RANGE(entropy, rows * 4, "frx_i8_ce_entropy: entropy");
+  FRX_CHECK_RANGE(lse, rows * 4, "frx_i8_ce_entropy: lse");
+  FRX_CHECK_RANGE(log_probs, rows * 4, "frx_i8_ce_entropy: log_probs");
   I8Operands op;
   int64_t used = 0;
   int rc = prepare_i8("frx_i8_ce_entropy", hidden, hidden_dtype, ld_hidden, hidden_scale, weight, ld_weight,
