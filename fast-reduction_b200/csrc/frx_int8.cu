@@ -24,7 +24,8 @@
 
 namespace frx {
 
-constexpr int64_t kI8MaxK = 131071;
+constexpr int64_t kI8MaxK = FRX_I8_MAX_K;
+static_assert(kI8MaxK * 128 * 128 < (1ll << 31) && (kI8MaxK + 1) * 128 * 128 >= (1ll << 31), "largest exact int32 sum");
 
 // ------------------------------------------------------------------------------------ quantisation
 // Eight consecutive values of a row as they lie in memory. max_bits folds the bits of |x| into a running
@@ -602,7 +603,7 @@ struct Int8CEPartialsEpilogue {
 //   storing   1 token 84 : 145, 11 : 16    64 tokens 92 : 113, 13 : 17     128 tokens 110 : 124, 16 : 19
 //   scoring   1 token 93 : 152, 18 : 23    64 tokens 105 : 125, 21 : 22    128 tokens 136 : 130, 27 : 21
 constexpr int kFewMaxTokens = 128;
-constexpr int kFewMaxScored = 64;
+constexpr int kFewMaxScored = FRX_I8_FEW_ROWS;
 constexpr int kFewWBytes = 128 * 128;
 constexpr int kFewThreads = 192;
 constexpr int kFewSmemBudget = 115712;  // of 228 KiB per SM for two CTAs, each with 1 KiB for the system

@@ -35,7 +35,7 @@
 
 namespace frx {
 
-constexpr int kVfyChunk = 2048;  // least columns per statistics partial (up to 7 of a first one lie before the row)
+constexpr int kVfyChunk = FRX_VERIFY_CHUNK;  // least columns per statistics partial (up to 7 of a first one lie before the row)
 constexpr int kVfyThreads = 256;
 constexpr int kVfyWarps = kVfyThreads / 32;
 constexpr int kVfyMaxCluster = 8;

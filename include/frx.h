@@ -75,6 +75,11 @@ extern "C" {
 #define FRX_STATUS_CHECK_FAILED 32 /* a device-side invariant check of a checked build failed */
 #define FRX_STATUS_BAD_OFFSETS 64  /* draft offsets that do not start at 0, decrease or pass the drafts */
 
+/* Sizes that a caller needs for the 8-bit head and the draft verification. */
+#define FRX_I8_MAX_K 131071   /* longest row of 8-bit codes whose products cannot overflow an int32 sum */
+#define FRX_I8_FEW_ROWS 64    /* up to so many rows frx_i8_ce_entropy makes one partial per 128 columns */
+#define FRX_VERIFY_CHUNK 2048 /* columns per workspace entry of frx_verify_drafts */
+
 /* ABI version of the loaded library (FRX_ABI_VERSION it was built with). */
 FRX_API int frx_abi_version(void);
 
@@ -311,7 +316,7 @@ FRX_API int frx_quantize_i8(const void* x, int dtype, int64_t ld_x, int64_t rows
 
 /*
  * out[r, j] = (sum_c xc[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]), with xc and weight [cols, k]
- * signed 8-bit codes: exact int32 sums (k <= 131071), scaled in fp32 and rounded once to out_dtype (BF16, F16 or
+ * signed 8-bit codes: exact int32 sums (k <= FRX_I8_MAX_K), scaled in fp32 and rounded once to out_dtype (BF16, F16 or
  * F32; any ld_out >= cols and any alignment of the element type).
  *   x_dtype    FRX_DTYPE_I8: x holds the codes, x_scale [rows] their scales. FRX_DTYPE_BF16, _F16 or _F32: x is
  *              quantised as by frx_quantize_i8 into the workspace first (x_scale is not read)
@@ -329,11 +334,11 @@ FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x
 /*
  * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
  * HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
- * frx_finalize, launch_rows rows at a time (up to 64 rows: all at once). Logits, and sum * weight_scale, are
+ * frx_finalize, launch_rows rows at a time (up to FRX_I8_FEW_ROWS rows: all at once). Logits, and sum * weight_scale, are
  * expected above -1e38; what is below (a bias of -inf) counts as masked. Operands as in frx_gemm_i8, target
  * rules as in frx_finalize.
  *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
- *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to 64 rows
+ *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to FRX_I8_FEW_ROWS rows
  *              16 * ceil(vocab_size / 128) * rows bytes
  * No counterpart in the reference.
  */
@@ -363,7 +368,7 @@ FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_h
  *                bad ones set FRX_STATUS_BAD_OFFSETS
  *   draft_probs  [n_drafts, vocab] (BF16, F16 or F32, row stride ld_draft_probs) or NULL
  *   temperature  [batch] or NULL (then temperature_all)
- *   workspace    at least 4 * (n_drafts + batch) * ceil((vocab + 7) / 2048) floats, 16-byte aligned; its contents
+ *   workspace    at least 4 * (n_drafts + batch) * ceil((vocab + 7) / FRX_VERIFY_CHUNK) floats, 16-byte aligned; its contents
  *                need not be kept between calls, and calls that overlap need one each
  *   accepted     [batch] number of accepted drafts
  *   tokens, log_probs  [n_drafts + batch], at the rows of the logits: the emitted tokens and their log p_i

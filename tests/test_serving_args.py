@@ -245,3 +245,27 @@ def test_forward_mode_tangents_are_refused():
                 fn(forward_ad.unpack_dual(dual).primal)
         with pytest.raises(ValueError, match="CUDA"):
             fn(dual)
+
+
+def test_sizes_shared_with_the_library():
+    """The limits that size workspaces in Python are those of the header that the kernels are compiled with, and the
+    library asks for the workspaces that Python makes at their borders."""
+    import re
+    from pathlib import Path
+
+    nat, lib = _lib()
+    header = (Path(__file__).resolve().parents[1] / "include" / "frx.h").read_text()
+    for name in ("FRX_I8_MAX_K", "FRX_I8_FEW_ROWS", "FRX_VERIFY_CHUNK", "FRX_DTYPE_I8", "FRX_STATUS_CHECK_FAILED",
+                 "FRX_STATUS_BAD_OFFSETS"):
+        assert int(re.search(rf"#define {name} (\d+)", header).group(1)) == getattr(nat, name), name
+    for rows in (nat.FRX_I8_FEW_ROWS - 1, nat.FRX_I8_FEW_ROWS, nat.FRX_I8_FEW_ROWS + 1, 300):
+        per = 128 if rows <= nat.FRX_I8_FEW_ROWS else 256
+        need = 16 * rows * ((1000 + per - 1) // per)
+        rc = lib.frx_i8_ce_entropy(A, nat.FRX_DTYPE_I8, 64, B, C, 64, D, None, 0, A, rows, 1000, 64, -100, rows, B,
+                                   need - 1, A, A, None, A, None, None)
+        assert rc == nat.FRX_ERR_INVALID_ARG and f"with {need} bytes".encode() in lib.frx_last_error()
+    for v in (1, nat.FRX_VERIFY_CHUNK - 7, nat.FRX_VERIFY_CHUNK - 6, 128256):
+        chunks = (v + 6) // nat.FRX_VERIFY_CHUNK + 1
+        rc = lib.frx_verify_drafts(A, 0, v, B, B, B, B, None, 1, 0, None, 1.0, 2, 3, v, C, 4 * 5 * chunks - 1, D, D, D, None,
+                                   None)
+        assert rc == nat.FRX_ERR_INVALID_ARG and f"4 * 5 * {chunks} floats".encode() in lib.frx_last_error()
