@@ -543,3 +543,35 @@ def test_results_of_scoring_are_tensors_of_their_own(rows):
         out[2].zero_()
         loss.backward()
         assert torch.equal(a.grad, out[1])
+
+
+@pytest.mark.parametrize("rows", [1, 33, 64, 128])
+@pytest.mark.parametrize("v", [37889, 128256])
+@pytest.mark.parametrize("k", [100, 1000])
+def test_few_tokens_with_many_tiles_per_cta(rows, v, k):
+    """Above 296 tiles of 128 entries a CTA of the few-token kernels takes several, through both accumulators, a ring of K
+    steps that wraps inside a tile and across tiles, and the same slots again. Without a bias and with one that masks
+    whole tiles, warps' quarters of a tile and single entries."""
+    from fast_reduction import int8_ce_entropy, int8_linear
+
+    x, w, ws, b = make(rows, k, v, torch.bfloat16, rows + k, torch.float32)
+    t = torch.randint(0, v, (rows,), device=DEV, generator=_gen(4))
+    t[0] = v - 1
+    c, s = ref_quantize(x)
+    masked = torch.rand(v, device=DEV, generator=_gen(1)) < 0.3
+    tile = torch.arange(v, device=DEV) // 128
+    masked |= (tile % 7 == 3) | ((tile % 5 == 1) & (torch.arange(v, device=DEV) % 128 < 32))
+    masked[t] = False
+    b[masked] = -float("inf")
+    for bias, keep in ((None, torch.ones_like(masked)), (b, ~masked)):
+        y = int8_linear(x, w, ws, bias=bias, out_dtype=torch.float32)
+        z, mag = ref_logits(c, s, w[keep], ws[keep], None if bias is None else bias[keep])
+        assert_logits(y[:, keep], z, mag)
+        assert (y[:, ~keep] == -float("inf")).all()
+        assert torch.equal(y, int8_linear(x, w, ws, bias=bias, out_dtype=torch.float32))
+        got = int8_ce_entropy(x, w, ws, t, bias=bias)
+        ce_r, ent_r, tol_ce, tol_ent = ref_score(z, mag, torch.cumsum(keep, 0)[t] - 1)
+        assert ((got[0].double() - ce_r).abs() <= tol_ce).all()
+        assert ((got[1].double() - ent_r).abs() <= tol_ent).all()
+        for _ in range(5):
+            assert all(torch.equal(a, e) for a, e in zip(int8_ce_entropy(x, w, ws, t, bias=bias), got))
