@@ -849,12 +849,25 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
 }
 
 // CTAs per sequence: many for few sequences, whose columns they share; fewer when the batch fills the GPU anyway,
-// since each CTA of a cluster waits for the decision. Sequences with draft probabilities, us with 8, 4, 2 and 1 CTAs:
-//   V = 128256, 0 to 7 drafts   16: 31, 35    48: 48, 55    64: 55, 57, 63, 92    96: 84, 78
-//   V = 32000, 4 drafts         256: 102, 75, 66, 74
-inline int verify_cluster(int64_t batch, int64_t vocab, int sms) {
+// since each CTA of a cluster waits for the decision. Three CTAs fit an SM. A batch that draws in every sequence is fastest
+// when all its clusters are resident together; greedy sequences leave early, so that a batch of mixed temperatures is
+// faster with up to 4 per SM. A temperature for all tells the two apart, temperatures of each do not. us with 8, 4, 2 and 1
+// CTAs, logits in bf16, 4 drafts per sequence (0 to 7 drafts: within 10 %, the same order but for one near tie):
+//                  V = 32000                                    V = 128256
+//   sequences      with draft probabilities    without          with draft probabilities      without
+//   32             20, 20, 24, 32              16, 16, 18, 21   37, 40, 54, 83                28, 29, 34, 46
+//   64             34, 27, 29, 37              29, 19, 20, 23   67, 61, 67, 91                51, 42, 45, 55
+//   96             44, 33, 35, 38              34, 24, 25, 26   88, 79, 89, 104               65, 56, 60, 69
+//   128            57, 45, 36, 40              46, 37, 27, 28   113, 105, 117, 133            86, 83, 77, 82
+//   192            80, 56, 48, 54              63, 44, 36, 38   160, 139, 135, 157            122, 102, 93, 102
+//   256            105, 75, 66, 61             87, 61, 52, 44   218, 191, 182, 183            171, 146, 134, 127
+//   512            204, 138, 114, 111          168, 111, 91, 85 396, 329, 300, 314            304, 245, 213, 217
+// A quarter of the sequences greedy: 64 of 0 to 7 drafts, V = 128256, fp32 probabilities 55, 58, 62, 92; 256 of 4, V = 32000,
+// fp32 logits, bf16 probabilities 104, 76, 67, 73.
+inline int verify_cluster(int64_t batch, int64_t vocab, int sms, bool all_draw) {
+  const int limit = (all_draw ? 3 : 4) * sms;
   int ctas = kVfyMaxCluster;
-  while (ctas > 1 && (batch * ctas > 4 * sms || vocab <= 256 * kVfyWarps * (ctas / 2))) ctas /= 2;
+  while (ctas > 1 && (batch * ctas > limit || vocab <= 256 * kVfyWarps * (ctas / 2))) ctas /= 2;
   return ctas;
 }
 
@@ -863,7 +876,7 @@ static int launch_verify(VerifyArgs& a, cudaStream_t stream) {
   int sms = 0;
   int rc = sm_count(&sms);
   if (rc) return rc;
-  const int ctas = verify_cluster(a.batch, a.vocab, sms);
+  const int ctas = verify_cluster(a.batch, a.vocab, sms, a.temperature == nullptr && a.temperature_all >= kVfyMinTemp);
   FRX_REQUIRE(a.batch * ctas < (1ll << 31), FRX_ERR_INVALID_ARG, "frx_verify_drafts: too many sequences (%lld)",
               (long long)a.batch);
   // a warp's columns in at most kVfyMaxGroups groups

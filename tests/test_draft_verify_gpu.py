@@ -439,3 +439,14 @@ def test_tensor_level_call_refuses_tensors_of_the_host():
             ops.verify_drafts(*args)
     with pytest.raises(ValueError, match="workspace"):
         ops.verify_drafts(*good[:8], torch.empty(1, device=DEV).expand(20), *good[9:])
+
+
+@pytest.mark.parametrize("batch,v", [(56, 9001), (64, 9001), (120, 4500), (128, 4500), (240, 2100), (256, 2100), (600, 300)])
+def test_batches_at_the_borders_of_the_cluster_sizes(batch, v):
+    """One temperature for all and the same one for each take clusters of other sizes; the decisions are the same."""
+    counts = [(5 * b + 3) % 4 for b in range(batch)]
+    for probs in (torch.float32, None):
+        args = make(counts, v, torch.bfloat16, batch, probs)
+        one = check(*args, temps=0.7)
+        each = check(*args, temps=torch.full((batch,), 0.7, device=DEV))
+        assert torch.equal(one[0], each[0]) and torch.equal(one[1], each[1])
