@@ -171,7 +171,16 @@ def status_word(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     w = _status_words.get(idx)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        dev = torch.device("cuda", idx)
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                # Zeroed on a stream outside the capture: as a node of the graph every replay would clear the bits
+                # that other launches have set, and until the first one they would be whatever the memory held.
+                w = torch.empty(1, dtype=torch.int32, device=dev)
+                with torch.cuda.stream(torch.cuda.Stream(dev)):
+                    w.zero_()
+            else:
+                w = torch.zeros(1, dtype=torch.int32, device=dev)
         _status_words[idx] = w
     return w
 

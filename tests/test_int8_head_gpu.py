@@ -575,3 +575,40 @@ def test_few_tokens_with_many_tiles_per_cta(rows, v, k):
         assert ((got[1].double() - ent_r).abs() <= tol_ent).all()
         for _ in range(5):
             assert all(torch.equal(a, e) for a, e in zip(int8_ce_entropy(x, w, ws, t, bias=bias), got))
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from fast_reduction import _native as nat, int8_ce_entropy
+dev = torch.device("cuda", 0)
+x, ws = torch.randn(4, 64, device=dev), torch.ones(300, device=dev)
+w, t = torch.randint(-127, 128, (300, 64), device=dev, dtype=torch.int8), torch.tensor([0, 1, 2, 3], device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ce, _, _ = int8_ce_entropy(x, w, ws, t)
+assert nat.read_status(dev) == 0
+bad = t.clone()
+bad[1] = 300
+want = int8_ce_entropy(x, w, ws, bad)[0]
+graph.replay()
+assert nat.read_status(dev) == nat.FRX_STATUS_BAD_TARGET
+assert nat.read_status(dev) == 0
+assert torch.equal(ce[[0, 2, 3]], want[[0, 2, 3]]) and ce.isfinite().all()
+t.fill_(-5)
+graph.replay()
+assert nat.read_status(dev) == nat.FRX_STATUS_BAD_TARGET and ce.isnan().all()
+"""
+
+
+def test_first_call_of_a_process_captured_in_a_graph():
+    """Replays neither clear what other calls reported nor need a call before the capture."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    repo = Path(__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=repo, capture_output=True, text=True, timeout=300,
+                         env=dict(os.environ, PYTHONPATH=str(repo / "fast-reduction_b200")))
+    assert out.returncode == 0, out.stderr[-2000:]
