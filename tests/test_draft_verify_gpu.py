@@ -450,3 +450,36 @@ def test_batches_at_the_borders_of_the_cluster_sizes(batch, v):
         one = check(*args, temps=0.7)
         each = check(*args, temps=torch.full((batch,), 0.7, device=DEV))
         assert torch.equal(one[0], each[0]) and torch.equal(one[1], each[1])
+
+
+def test_two_threads_and_streams_at_once():
+    """Two host threads, each on its own stream, verify batches that share the GPU, one of them beside the head's product."""
+    import threading
+
+    from fast_reduction import int8_linear, quantize_int8, verify_drafts
+
+    work = [make([4, 0, 7, 2] * n, v, torch.bfloat16, n, probs) for n, v, probs in
+            ((3, 20000, torch.float32), (40, 5000, None))]
+    temps = [0.8, torch.tensor([0.0, 0.6, 1.0, 1.3] * 40, device=DEV)]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    codes, scale = quantize_int8(torch.randn(9000, 256, device=DEV, generator=g))
+    h = torch.randn(200, 256, device=DEV, generator=g)
+    want = [check(*w, temps=t) for w, t in zip(work, temps)]
+    logits = int8_linear(h, codes, scale)
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(40):
+                y = int8_linear(h, codes, scale) if i else logits
+                got = verify_drafts(*work[i], temperature=temps[i])
+                if not (torch.equal(y, logits) and all(torch.equal(a, b) for a, b in zip(got, want[i]))):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(120)
+    assert not bad
