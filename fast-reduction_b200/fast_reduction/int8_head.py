@@ -168,7 +168,8 @@ def int8_ce_entropy(
     chunk = gk._chunk_rows(chunk_size, B)
     dev = x.device
     # three tensors: views of one would share a version counter, and each would keep the memory of all
-    ce, ent, logp = (torch.empty(B, device=dev, dtype=torch.float32) for _ in range(3))
+    ce = torch.empty(B, device=dev, dtype=torch.float32)
+    ent, logp = torch.empty_like(ce), torch.empty_like(ce)
     if B:
         V = w.shape[0]
         if B <= nat.FRX_I8_FEW_ROWS:

@@ -494,14 +494,15 @@ def _call(name: str, entry: str, dev: torch.device, *args) -> None:
 
 
 def _one_device(first: torch.Tensor, *rest: torch.Tensor | None) -> torch.device:
-    """_require_cuda, with its loop left to the case that it refuses."""
-    dev = first.device
-    if dev.type == "cuda":
+    """_require_cuda, with its loop left to the case that it refuses (a device's number is read in half the time of a
+    torch.device; the CPU's is -1)."""
+    index = first.get_device()
+    if index >= 0:
         for t in rest:
-            if t is not None and t.device != dev:
+            if t is not None and t.get_device() != index:
                 break
         else:
-            return dev
+            return first.device
     return _require_cuda(first, *rest)
 
 
@@ -522,10 +523,9 @@ def _is_vector(t: torch.Tensor, dtype: torch.dtype, n: int) -> bool:
     return t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
 
 
-def _leading(t: torch.Tensor, name: str) -> int:
-    """Row stride of a matrix for the C entry points. A dimension of one may come with any stride (torch calls that
+def _leading(t: torch.Tensor, rows: int, cols: int, name: str) -> int:
+    """Row stride of a [rows, cols] matrix for the C entry points. A dimension of one may come with any stride (torch calls that
     contiguous); otherwise columns lie next to each other and rows do not overlap."""
-    rows, cols = t.shape
     ld, unit = t.stride()
     if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
         raise ValueError(f"{name} must have unit column stride and rows that do not overlap, got shape {tuple(t.shape)} "
@@ -550,7 +550,7 @@ def quantize_i8(x: torch.Tensor, codes: torch.Tensor, scale: torch.Tensor) -> No
     if codes.shape != x.shape or scale.shape != x.shape[:1] or not scale.is_contiguous():
         raise ValueError("codes must have x's shape and scale one value per row")
     rows, cols = x.shape
-    ldx, ldc = _leading(x, "x"), _leading(codes, "codes")
+    ldx, ldc = _leading(x, rows, cols, "x"), _leading(codes, rows, cols, "codes")
     lib = nat.load()
     with torch.cuda.device(dev):
         rc = _launch("quantize_i8", dev, lambda: lib.frx_quantize_i8(
@@ -575,7 +575,7 @@ def _i8_operands(x, x_scale, weight, weight_scale, bias, *others):
     cols, wk = weight.shape
     if wk != k:
         raise ValueError(f"row length mismatch: x {tuple(x.shape)} vs weight {tuple(weight.shape)}")
-    ldx, ldw = _leading(x, "x"), _leading(weight, "weight")
+    ldx, ldw = _leading(x, rows, k, "x"), _leading(weight, cols, k, "weight")
     if not _is_vector(weight_scale, torch.float32, cols):
         raise ValueError(f"weight_scale must be contiguous float32 [{cols}], got {weight_scale.dtype} "
                          f"{tuple(weight_scale.shape)}")
@@ -607,7 +607,7 @@ def gemm_i8(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor,
     if odt is None or out.shape != (rows, cols):
         raise ValueError(f"out must be bfloat16, float16 or float32 [{rows}, {cols}], got {out.dtype} {tuple(out.shape)}")
     _call("gemm_i8", "frx_gemm_i8", dev, *operands, rows, cols, k, *_room(workspace, torch.uint8), out.data_ptr(),
-          _leading(out, "out"), odt)
+          _leading(out, rows, cols, "out"), odt)
 
 
 def i8_ce_entropy(x: torch.Tensor, x_scale: torch.Tensor | None, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -637,14 +637,14 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.T
     if dt is None or rows != n + batch:
         raise ValueError(f"logits must be bfloat16, float16 or float32 [{n + batch}, V], got {logits.dtype} "
                          f"{tuple(logits.shape)}")
-    ldl = _leading(logits, "logits")
+    ldl = _leading(logits, rows, vocab, "logits")
     qptr, qdt, ldq = None, 0, 0
     if draft_probs is not None:
         qdt = _LOGITS_DTYPES.get(draft_probs.dtype)
         if qdt is None or draft_probs.shape != (n, vocab):
             raise ValueError(f"draft_probs must be bfloat16, float16 or float32 [{n}, {vocab}], got {draft_probs.dtype} "
                              f"{tuple(draft_probs.shape)}")
-        qptr, ldq = draft_probs.data_ptr(), _leading(draft_probs, "draft_probs")
+        qptr, ldq = draft_probs.data_ptr(), _leading(draft_probs, n, vocab, "draft_probs")
     if not _is_vector(drafts, torch.int64, n) or not _is_vector(cu_drafts, torch.int64, batch + 1):
         raise ValueError("drafts and cu_drafts must be contiguous int64 vectors")
     if not _is_vector(uniforms, torch.float32, n):

@@ -197,7 +197,7 @@ def test_tensor_level_calls_refuse_layouts_that_pass_their_memory():
             ops._room(bad, torch.uint8)
     for bad in (torch.zeros(1, 10).expand(4, 10), torch.zeros(10, 4).t()):
         with pytest.raises(ValueError, match="out must"):
-            ops._leading(bad, "out")
+            ops._leading(bad, 4, 10, "out")
     z, q, d = torch.zeros(5, 20), torch.full((3, 20), 0.05), torch.zeros(3, dtype=torch.int64)
     cu, u, f, e = torch.tensor([0, 1, 3]), torch.zeros(3), torch.zeros(2), torch.zeros(20)
 
