@@ -11,11 +11,12 @@
 // kind::i8 hold it exactly and the result does not depend on the order of the products.
 //
 // What bounds them (one B200; 6.56 TB/s is what a copy reaches):
-//   quantisation    HBM: 128256 x 4096 fp32 367 us (7.2 TB/s), bf16 329 us (4.8 TB/s: two dependent phases per row)
+//   quantisation    fp32 HBM: 128256 x 4096 364 us (7.2 TB/s); bf16 and fp16 issue slots (0.82 and 0.84 instructions per cycle
+//                   and scheduler, HBM 52 %): 316 us (5.0 TB/s) and 275 us
 //   few tokens      HBM: 1 token x 4096 x 128256 84 us (6.2 TB/s of weight), 64 tokens 92 us
 //   many tokens     the tensor pipe's power and the L2's bandwidth to the SMs together: a 256 x 256 tile moves
-//                   512 bytes per K and SM pair, 12 TB/s. 4096 tokens x 4096 x 32768 stored 406 us (2.7 POP/s),
-//                   x 128256 scored 1.44 ms (3.0 POP/s, tensor pipe 90 % active at 1.53 GHz)
+//                   512 bytes per K and SM pair, 12 TB/s. 4096 tokens x 4096 x 32768 stored 418 us (2.6 POP/s),
+//                   x 128256 scored 1.45 ms (3.0 POP/s, tensor pipe 91 % active at 1.55 GHz)
 #include <cstring>
 #include <type_traits>
 
@@ -599,9 +600,10 @@ struct Int8CEPartialsEpilogue {
 // quantisation. The ring holds at most 4 steps, 128 KB of weight in flight per SM (1 token: 88.7 us with 6 steps, 84.1
 // with 4, 86 with 3, 97 with 2), and the weight is marked to leave the L2 first, so that the tokens stay
 // (64 tokens: 96 -> 92 us).
-// Against the CTA-pair core, us at 4096 x 128256 and 1024 x 32000 (its loads of token rows that do not exist are slow):
-//   storing   1 token 84 : 145, 11 : 16    64 tokens 92 : 113, 13 : 17     128 tokens 110 : 124, 16 : 19
-//   scoring   1 token 93 : 152, 18 : 23    64 tokens 105 : 125, 21 : 22    128 tokens 136 : 130, 27 : 21
+// Against the CTA-pair core, us at 4096 x 128256 and 1024 x 32000, bf16 in and out, inputs larger than the L2 (its loads of
+// token rows that do not exist are slow):
+//   storing   1 token 83 : 132, 11 : 16    64 tokens 87 : 98, 12 : 16      128 tokens 95 : 106, 15 : 16
+//   scoring   1 token 94 : 140, 17 : 21    64 tokens 98 : 105, 20 : 22     128 tokens 124 : 109, 28 : 20
 constexpr int kFewMaxTokens = 128;
 constexpr int kFewMaxScored = FRX_I8_FEW_ROWS;
 constexpr int kFewWBytes = 128 * 128;

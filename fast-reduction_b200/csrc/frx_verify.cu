@@ -22,10 +22,12 @@
 //           number falls in is a comparison over up to V borders, and sums in 32 bits would move each
 //           border by 1e-7, enough to change a token about once in a hundred rows at V = 128256. Acceptance is one
 //           comparison, which the statistics' fp32 sum decides unless the two sides are closer than that sum's
-//           error bound (stats_sum_error, 7e-5; one draft in some ten thousand): then the row is summed in 64 bits. It is
-//           bound by issue slots and the 64-bit pipe (64 lanes per SM and clock), so the exponential is a
-//           short one of its own (exp2_scaled below). 64 sequences of V = 128256 with draft probabilities: 55 us
-//           in all; per cluster 5 us for the decision, 7 for a pass over a row, 3 for the search.
+//           error bound (stats_sum_error, 7e-5; one draft in some ten thousand): then the row is summed in 64 bits.
+//           It is bound by latency: a cluster waits for its first CTA's decision (the largest stall is the barrier,
+//           issue slots and the 64-bit pipe are below 30 % on average), and its passes are long chains of
+//           64-bit operations, so the exponential is a short one of its own (exp2_scaled below). 64 sequences of
+//           V = 128256 with draft probabilities: 56 us in all; per cluster 5 us for the decision, 7 for a pass over a
+//           row, 3 for the search.
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -852,7 +854,7 @@ __global__ void __launch_bounds__(kVfyThreads, 3) verify_sample_kernel(const __g
 // since each CTA of a cluster waits for the decision. Three CTAs fit an SM. A batch that draws in every sequence is fastest
 // when all its clusters are resident together; greedy sequences leave early, so that a batch of mixed temperatures is
 // faster with up to 4 per SM. A temperature for all tells the two apart, temperatures of each do not. us with 8, 4, 2 and 1
-// CTAs, logits in bf16, 4 drafts per sequence (0 to 7 drafts: within 10 %, the same order but for one near tie):
+// CTAs, logits in bf16, 4 drafts per sequence (0 to 7 drafts: the same best ones, but 2 for 128 with probabilities at V = 128256):
 //                  V = 32000                                    V = 128256
 //   sequences      with draft probabilities    without          with draft probabilities      without
 //   32             20, 20, 24, 32              16, 16, 18, 21   37, 40, 54, 83                28, 29, 34, 46

@@ -69,9 +69,10 @@ def verify_drafts(
 
     Returns (accepted int64 [B], tokens int64 [N + B], log_probs fp32 [N + B]): at the logits rows, the tokens
     emitted there and their log p_i (greedy: at temperature 1); -1 and 0 where nothing is emitted. A row that
-    leaves nothing to draw emits -1 with log-probability -inf. Decisions are taken in 64 bits. No host
-    synchronisation. Nothing here is differentiable: logits or draft_probs that require a gradient are refused while
-    gradients are enabled."""
+    leaves nothing to draw emits -1 with log-probability -inf. Decisions are taken in 64 bits (in a draw, p below e^-680 of
+    the row's largest counts as 0); log_probs come from sums in fp32. No host synchronisation. Nothing here is
+    differentiable: logits or draft_probs that require a gradient (while gradients are enabled) or have a forward-mode
+    tangent are refused."""
     drafts, cu = _ids(draft_tokens, "draft_tokens"), _ids(cu_drafts, "cu_drafts")
     n, batch = drafts.numel(), cu.numel() - 1
     if batch < 0:

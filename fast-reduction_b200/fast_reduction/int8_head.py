@@ -9,7 +9,7 @@ vocabulary row, products on the int8 tensor cores.
 Quantisation is symmetric: scale_r = max |x_r| / 127 (fp32), code = the integer nearest to x / scale_r.
 The sums of code products are exact (int32); scales and bias are applied in fp32 and each output is
 rounded once. Nothing here is differentiable: the results carry no gradient, and inputs that require one
-are refused while gradients are enabled.
+(while gradients are enabled) or have a forward-mode tangent are refused.
 
 No counterpart in the reference, whose head is bf16 / fp16 / fp32 (fast_reduction/gemm_kernel.py:276-356);
 int8_ce_entropy returns what its gemm_fused_ce_entropy does.
@@ -153,9 +153,11 @@ def int8_ce_entropy(
     hidden_scale: Optional[Tensor] = None,
 ) -> Tuple[Tensor, Tensor, Tensor]:
     """(ce_loss, entropy, log_probs), each fp32 and shaped like ``hidden.shape[:-1]``, of the logits
-    int8_linear would give in fp32, which never reach HBM. Operands as in int8_linear; target, chunk_size and
+    int8_linear would give in fp32 (but for the order of the two scales' products, a step or two of fp32), which never
+    reach HBM. Operands as in int8_linear; target, chunk_size and
     ignore_index as in gemm_fused_ce_entropy (ignored rows: ce = log_probs = 0, entropy kept; a target
-    outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET). A bias of -inf masks its vocabulary entry."""
+    outside [0, V) gives NaN and sets FRX_STATUS_BAD_TARGET). A bias of -inf masks its vocabulary entry,
+    as do all logits below -1e38; others are expected below 1e38, also before ``hidden_scale`` is multiplied in."""
     x, x_scale, w, w_scale, bias = _prepare(hidden, weight_codes, weight_scale, bias, hidden_scale)
     B = x.shape[0]
     if target.numel() != B:

@@ -316,8 +316,8 @@ FRX_API int frx_quantize_i8(const void* x, int dtype, int64_t ld_x, int64_t rows
 
 /*
  * out[r, j] = (sum_c xc[r, c] weight[j, c]) x_scale[r] weight_scale[j] (+ bias[j]), with xc and weight [cols, k]
- * signed 8-bit codes: exact int32 sums (k <= FRX_I8_MAX_K), scaled in fp32 and rounded once to out_dtype (BF16, F16 or
- * F32; any ld_out >= cols and any alignment of the element type).
+ * signed 8-bit codes: exact int32 sums (k <= FRX_I8_MAX_K), scaled in fp32, x_scale first, and rounded once to out_dtype
+ * (BF16, F16 or F32; any ld_out >= cols and any alignment of the element type). sum * x_scale has to be a finite float.
  *   x_dtype    FRX_DTYPE_I8: x holds the codes, x_scale [rows] their scales. FRX_DTYPE_BF16, _F16 or _F32: x is
  *              quantised as by frx_quantize_i8 into the workspace first (x_scale is not read)
  *   codes      16-byte aligned bases, row strides that are multiples of 16
@@ -332,10 +332,10 @@ FRX_API int frx_gemm_i8(const void* x, int x_dtype, int64_t ld_x, const float* x
                         int out_dtype, int* status, void* stream);
 
 /*
- * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits frx_gemm_i8 would give, which never reach
- * HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
+ * ce, entropy, lse, log_probs (any may be NULL) of the fp32 logits of frx_gemm_i8 (but for the order in which the two
+ * scales are multiplied in, a step or two of fp32), which never reach HBM: the product's epilogue reduces them to partials like frx_fwd_partials' and they are merged as by
  * frx_finalize, launch_rows rows at a time (up to FRX_I8_FEW_ROWS rows: all at once). Logits, and sum * weight_scale, are
- * expected above -1e38; what is below (a bias of -inf) counts as masked. Operands as in frx_gemm_i8, target
+ * expected between -1e38 and 1e38; what is below (a bias of -inf) counts as masked. Operands as in frx_gemm_i8, target
  * rules as in frx_finalize.
  *   workspace  16-byte aligned; that of frx_gemm_i8 (0 bytes for FRX_DTYPE_I8) plus
  *              16 * ceil(vocab_size / 256) * min(rows, launch_rows) bytes, for up to FRX_I8_FEW_ROWS rows
@@ -357,7 +357,8 @@ FRX_API int frx_i8_ce_entropy(const void* hidden, int hidden_dtype, int64_t ld_h
  * and the sequence emits its accepted drafts and one more token, drawn as the first j with w_j > 0 and
  * sum_{k<=j} w_k > final_uniforms[b] * sum_k w_k, where w = max(p - q, 0) at the rejected draft's row (NULL:
  * p without the rejected token; p itself when nothing is left), or p of the last row after full acceptance.
- * Decisions are taken in 64 bits. T < 1e-6 (or NaN) is greedy: a draft must equal its row's argmax
+ * Decisions are taken in 64 bits, with p below e^-680 of a row's largest as 0 in a draw; log_probs come from sums in fp32.
+ * T < 1e-6 (or NaN) is greedy: a draft must equal its row's argmax
  * (lowest index of a tie) and the argmax is emitted. T above 1e6 counts as 1e6. NaN logits count as -inf, +inf
  * as the largest finite float (16-bit logits: the largest bf16 value), negative or NaN draft probabilities
  * as 0; a row with nothing left to draw emits -1 with log-probability -inf.
