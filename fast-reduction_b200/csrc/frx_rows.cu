@@ -20,6 +20,10 @@ struct OnlineStat {
   float m, s, u;
 };
 
+// A rise of the maximum by more than 1e4 leaves nothing of what was below it. Held there, its product with s stays finite
+// behind masks of the lowest float, and infinity times a weight of 0 does not turn up as NaN. NaN stays NaN.
+__device__ __forceinline__ float bounded_fall(float d) { return d < -1e4f ? -1e4f : d; }
+
 __device__ __forceinline__ void online_merge(OnlineStat& a, const OnlineStat& b) {
   if (b.m == -INFINITY) return;
   if (a.m == -INFINITY) {
@@ -27,7 +31,7 @@ __device__ __forceinline__ void online_merge(OnlineStat& a, const OnlineStat& b)
     return;
   }
   const float M = fmaxf(a.m, b.m);
-  const float da = a.m - M, db = b.m - M;
+  const float da = bounded_fall(a.m - M), db = bounded_fall(b.m - M);
   const float ea = ex2_approx(da * kLog2e), eb = ex2_approx(db * kLog2e);
   a.u = fmaf(da, a.s, a.u) * ea + fmaf(db, b.s, b.u) * eb;
   a.s = a.s * ea + b.s * eb;
@@ -46,7 +50,7 @@ __device__ __forceinline__ void online_add(OnlineStat& st, const float (&v)[N], 
     if (i < n_valid) vm = fmaxf(vm, v[i]);
   if (vm > st.m) {
     if (st.m != -INFINITY) {
-      const float d = st.m - vm;
+      const float d = bounded_fall(st.m - vm);
       const float e = ex2_approx(d * kLog2e);
       st.u = fmaf(d, st.s, st.u) * e;
       st.s *= e;

@@ -86,3 +86,25 @@ def test_rising_and_wide_range_logits(dtype):
     torch.testing.assert_close(lse.double(), lse_r, atol=1e-3, rtol=2e-6)
     torch.testing.assert_close(ce.double(), ce_r, atol=1e-3, rtol=2e-5)
     torch.testing.assert_close(ent.double(), ent_r, atol=2e-4, rtol=2e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_masks_of_the_lowest_value_before_live_logits(dtype, offset):
+    """Stretches of the type's lowest value (or -1e37) of any length in front of live logits have a weight of exactly 0."""
+    from fast_reduction.cute_cross_entropy import ce_entropy_fwd_with_lse
+
+    N = 40000
+    stretches = [(0, 1), (0, 8), (3, 700), (0, 4096), (256, 9000), (100, 39000), (0, N - 1)]
+    for fill in (torch.finfo(dtype).min, -1e37 if dtype != torch.float16 else -6e4):
+        x = torch.randn(len(stretches), N + offset, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3)) * 3
+        x = x.to(dtype)[:, offset:]
+        for r, (a, b) in enumerate(stretches):
+            x[r, a:b] = fill
+        t = torch.full((len(stretches),), N - 1, device=DEV)
+        ce, ent, lse = ce_entropy_fwd_with_lse(x, t)
+        ce_r, ent_r, lse_r = _ref(x, t)
+        tol = dict(atol=2e-4, rtol=2e-5)
+        torch.testing.assert_close(ce.double(), ce_r, **tol)
+        torch.testing.assert_close(ent.double(), ent_r, **tol)
+        torch.testing.assert_close(lse.double(), lse_r, **tol)
