@@ -181,7 +181,7 @@ def status_word(device: torch.device) -> torch.Tensor:
                     w.zero_()
             else:
                 w = torch.zeros(1, dtype=torch.int32, device=dev)
-        _status_words[idx] = w
+        w = _status_words.setdefault(idx, w)  # of two threads' first calls at once, one word stays for both
     return w
 
 

@@ -54,3 +54,35 @@ def test_threads_on_own_streams_match_serial_calls():
     for i, (got, want) in enumerate(zip(parallel, serial)):
         for name, a, b in zip(("ce", "entropy", "log_probs", "loss", "d_hidden", "d_weight"), got, want):
             assert torch.equal(a, b), (i, name)
+
+
+FIRST_CALLS = """
+import threading
+import torch
+from fast_reduction import _native as nat
+torch.zeros(1, device="cuda")
+gate, words = threading.Barrier(16), []
+
+def first():
+    gate.wait()
+    words.append(nat.status_word(torch.device("cuda", 0)).data_ptr())
+
+threads = [threading.Thread(target=first) for _ in range(16)]
+[t.start() for t in threads]
+[t.join(60) for t in threads]
+assert len(words) == 16 and set(words) == {nat.status_word(torch.device("cuda", 0)).data_ptr()}, words
+"""
+
+
+def test_first_calls_of_many_threads_share_one_status_word():
+    """A word of its own for one of them would be freed while launches, or a captured graph, still point to it."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    repo = Path(__file__).resolve().parents[1]
+    for _ in range(3):
+        out = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=repo, capture_output=True, text=True, timeout=300,
+                             env=dict(os.environ, PYTHONPATH=str(repo / "fast-reduction_b200")))
+        assert out.returncode == 0, out.stderr[-2000:]
